@@ -41,6 +41,8 @@ extern "C" {
 /* bits of the device status word (0 = fine) */
 #define SBATTN_ST_BAD_SEQLENS 1u /* sequence ends decrease, exceed the token count or max_seqlen         */
 #define SBATTN_ST_TIMEOUT 2u     /* a bounded wait inside a kernel gave up; results are invalid          */
+#define SBATTN_ST_BAD_PAGES 4u   /* cache: a page index outside the cache, or pieces / sizes that do not fit together */
+#define SBATTN_ST_NO_PAGES 8u    /* sbattn_cache_blocks: fewer free pages than the new tokens need       */
 
 /* element types of q, k, v, o, rem, do, drem, dq, dk, dv */
 #define SBATTN_BF16 0
@@ -177,6 +179,80 @@ unsigned long long sbattn_launch_count(void);
  * memory, out[2] = 0 before the call; the kernel writes the first entry, the longest sequence, and last out[2] = 1, so that the host can
  * wait for this word: a few microseconds sooner than for a copy and a stream synchronisation. */
 int sbattn_seq_bounds(const void* cu, int cu_width, int64_t n, int leading, int64_t* out, void* stream);
+
+/* ------------------------------------------------------------------------------------------------------------------
+ * Serving from a paged cache held in 8 bits.  No counterpart in the reference.
+ *
+ * A cache of one layer: codes k and v, float8 e4m3, [pages][kv_heads][page_tokens][row] with row = 32, 64 or 128, the smallest that
+ * holds head_dim (codes behind head_dim are zero), and a float32 scale per page and head: value = code * scale.  Token t of request r
+ * lies in page tables[r][t / page_tokens], place t % page_tokens. */
+
+/* One step of the block tables: tokens are added to or taken from every request.  All arrays are int32 on the device.
+ *   lengths[requests], new_tokens[requests]: tokens before the step; tokens to add (negative: to take away, from the end)
+ *   tables[requests][width] (rows table_stride apart): entries of pages that are added are written, the others are not touched
+ *   free_pages[pages]: a stack of free pages, free_count[0] of them; pages that come back are written above its top
+ * Outputs (none may overlap the inputs): lengths_out[requests], free_count_out[1]: the same after the step; ends[requests]: cumulative
+ * ends of the new tokens packed one request behind the other; slots[tokens]: page * page_tokens + place of each new token, -1 behind the
+ * last one; pieces[n_pieces][4]: (page, first new token, tokens that were in the page before, new tokens in it) of every page
+ * that new tokens go to, page -1 behind the last one.  n_pieces = sbattn_cache_pieces(...).
+ * Neither lengths nor free_count are changed: a step that is not wanted is dropped by not copying the outputs over them, and the same
+ * call again gives the same outputs.
+ * Too few pages (SBATTN_ST_NO_PAGES), a length below zero or above width * page_tokens, or more new tokens than `tokens`
+ * (SBATTN_ST_BAD_SEQLENS): nothing is added or taken away, ends are zero, slots and pages of pieces -1. */
+typedef struct SbBlocksParams {
+    int32_t requests, width, pages, page_tokens, tokens, n_pieces;
+    int64_t table_stride;
+    const int32_t *lengths, *new_tokens, *free_count;
+    int32_t *tables, *free_pages;
+    int32_t *lengths_out, *free_count_out, *ends, *slots, *pieces;
+    uint32_t* status;
+    void* stream;
+} SbBlocksParams;
+
+#define SBATTN_MAX_REQUESTS 4096
+
+int sbattn_cache_blocks(const SbBlocksParams* p);
+/* most pieces that `tokens` new tokens of `requests` requests can make */
+int64_t sbattn_cache_pieces(int64_t requests, int64_t tokens, int64_t page_tokens);
+
+typedef struct SbCacheParams {
+    int32_t dtype;          /* of q, k, v, o, rem: SBATTN_BF16 / F32 / F16                                */
+    int32_t heads;          /* query heads: a multiple of kv_heads (head h reads key/value head h / (heads / kv_heads)) */
+    int32_t kv_heads, head_dim, row, page_tokens, pages;
+    int32_t tokens;         /* rows of q, k, v, o                                                          */
+    int32_t requests, width, n_pieces, attend_current;
+    float inv_temp;
+    void *k_codes, *v_codes;             /* 16-byte aligned                                                */
+    float *k_scale, *v_scale;
+    int64_t k_stride, v_stride;          /* bytes from page to page, multiples of 16                       */
+    int64_t k_scale_stride, v_scale_stride; /* scales from page to page                                    */
+    SbMat q, k, v, o;       /* [H][T][D] (stride_b unused); append: k and v in; attend: q in, o out, v (may be NULL) in */
+    SbVec rem;              /* attend, out                                                                 */
+    const int32_t *pieces;  /* append: [n_pieces][4] of sbattn_cache_blocks                                */
+    const int32_t *tables;  /* attend: [requests][width], rows table_stride apart                          */
+    int64_t table_stride;
+    const int32_t *lengths; /* attend: tokens of every request, the rows of q included                     */
+    const int32_t *ends;    /* attend: cumulative ends of the rows of q; NULL: one row per request         */
+    void* workspace;        /* attend: sbattn_cached_workspace_bytes, 256-byte aligned                     */
+    size_t workspace_bytes;
+    uint32_t* status;
+    void* stream;
+} SbCacheParams;
+
+/* New keys and values go into their pages.  The scale of a page and head is a power of two, the smallest that keeps its largest finite
+ * value within e4m3's 448 (at least 2^-118); it grows when a larger value comes, and the tokens that are there are
+ * rounded to the new one.  Infinities and NaN become the NaN code.  A page may be named by one piece at a time only. */
+int sbattn_cache_append(const SbCacheParams* p);
+
+/* o, rem <- q and the cache: query row i of request r is one of its last tokens (the rows of a request are its last tokens in order) and
+ * sees the keys before it (and its own with attend_current).  With v (the new tokens' values, kv_heads) o + rem * v is written to o, rem
+ * rounded first.  Rows behind the last end: rem is zero, o is left alone.  A request of length 0 with a row of its own (ends NULL) likewise. */
+int sbattn_cached_fwd(const SbCacheParams* p);
+int sbattn_cached_workspace_bytes(const SbCacheParams* p, size_t* bytes);
+
+/* sizeof(SbBlocksParams), sizeof(SbCacheParams) */
+size_t sbattn_blocks_params_size(void);
+size_t sbattn_cache_params_size(void);
 
 #ifdef __cplusplus
 }

@@ -8,7 +8,7 @@ LIB_PATH = os.path.join(HERE, "libsbattn.so")
 
 SBATTN_BF16, SBATTN_F32, SBATTN_F16 = 0, 1, 2
 PATH_AUTO, PATH_SIMT, PATH_TENSOR = 0, 1, 2
-ST_BAD_SEQLENS, ST_TIMEOUT = 1, 2
+ST_BAD_SEQLENS, ST_TIMEOUT, ST_BAD_PAGES, ST_NO_PAGES = 1, 2, 4, 8
 
 
 class SbMat(ctypes.Structure):
@@ -36,11 +36,36 @@ class SbParams(ctypes.Structure):
     ]
 
 
+class SbBlocksParams(ctypes.Structure):
+    _fields_ = [
+        ("requests", ctypes.c_int32), ("width", ctypes.c_int32), ("pages", ctypes.c_int32), ("page_tokens", ctypes.c_int32),
+        ("tokens", ctypes.c_int32), ("n_pieces", ctypes.c_int32), ("table_stride", ctypes.c_int64), ("lengths", ctypes.c_void_p),
+        ("new_tokens", ctypes.c_void_p), ("free_count", ctypes.c_void_p), ("tables", ctypes.c_void_p), ("free_pages", ctypes.c_void_p),
+        ("lengths_out", ctypes.c_void_p), ("free_count_out", ctypes.c_void_p), ("ends", ctypes.c_void_p), ("slots", ctypes.c_void_p),
+        ("pieces", ctypes.c_void_p), ("status", ctypes.c_void_p), ("stream", ctypes.c_void_p),
+    ]
+
+
+class SbCacheParams(ctypes.Structure):
+    _fields_ = [
+        ("dtype", ctypes.c_int32), ("heads", ctypes.c_int32), ("kv_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32),
+        ("row", ctypes.c_int32), ("page_tokens", ctypes.c_int32), ("pages", ctypes.c_int32), ("tokens", ctypes.c_int32),
+        ("requests", ctypes.c_int32), ("width", ctypes.c_int32), ("n_pieces", ctypes.c_int32), ("attend_current", ctypes.c_int32),
+        ("inv_temp", ctypes.c_float), ("k_codes", ctypes.c_void_p), ("v_codes", ctypes.c_void_p), ("k_scale", ctypes.c_void_p),
+        ("v_scale", ctypes.c_void_p), ("k_stride", ctypes.c_int64), ("v_stride", ctypes.c_int64), ("k_scale_stride", ctypes.c_int64),
+        ("v_scale_stride", ctypes.c_int64), ("q", SbMat), ("k", SbMat), ("v", SbMat), ("o", SbMat), ("rem", SbVec),
+        ("pieces", ctypes.c_void_p), ("tables", ctypes.c_void_p), ("table_stride", ctypes.c_int64), ("lengths", ctypes.c_void_p),
+        ("ends", ctypes.c_void_p), ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t), ("status", ctypes.c_void_p),
+        ("stream", ctypes.c_void_p),
+    ]
+
+
 FLAG_FUSED_REMAINDER, FLAG_REMAINDER_IN_DV = 1, 2
 
 EXPORTS = ("sbattn_workspace_bytes", "sbattn_fwd", "sbattn_bwd", "sbattn_strerror", "sbattn_version",
            "sbattn_params_size", "sbattn_fwd_static", "sbattn_static_scratch_bytes", "sbattn_attention_weights",
-           "sbattn_launch_count", "sbattn_seq_bounds")
+           "sbattn_launch_count", "sbattn_seq_bounds", "sbattn_cache_blocks", "sbattn_cache_pieces", "sbattn_cache_append",
+           "sbattn_cached_fwd", "sbattn_cached_workspace_bytes", "sbattn_blocks_params_size", "sbattn_cache_params_size")
 
 _lib = None
 
@@ -79,8 +104,19 @@ def lib():
         L.sbattn_attention_weights.argtypes = [ctypes.POINTER(SbParams), ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64,
                                                ctypes.c_int64]
         L.sbattn_attention_weights.restype = ctypes.c_int
+        for name in ("sbattn_blocks_params_size", "sbattn_cache_params_size"):
+            getattr(L, name).restype = ctypes.c_size_t
+        for name, cls in (("sbattn_cache_blocks", SbBlocksParams), ("sbattn_cache_append", SbCacheParams), ("sbattn_cached_fwd", SbCacheParams)):
+            getattr(L, name).argtypes = [ctypes.POINTER(cls)]
+            getattr(L, name).restype = ctypes.c_int
+        L.sbattn_cached_workspace_bytes.argtypes = [ctypes.POINTER(SbCacheParams), ctypes.POINTER(ctypes.c_size_t)]
+        L.sbattn_cached_workspace_bytes.restype = ctypes.c_int
+        L.sbattn_cache_pieces.argtypes = [ctypes.c_int64] * 3
+        L.sbattn_cache_pieces.restype = ctypes.c_int64
         if L.sbattn_params_size() != ctypes.sizeof(SbParams):
             raise RuntimeError("libsbattn.so and its Python binding disagree about SbParams")
+        if L.sbattn_blocks_params_size() != ctypes.sizeof(SbBlocksParams) or L.sbattn_cache_params_size() != ctypes.sizeof(SbCacheParams):
+            raise RuntimeError("libsbattn.so and its Python binding disagree about the structures of the cache")
         _lib = L
     return _lib
 

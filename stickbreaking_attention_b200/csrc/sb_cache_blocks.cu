@@ -1,0 +1,161 @@
+// Block tables, slots and pieces of one serving step, built on the GPU from the requests' lengths: a stack allocator of pages whose every
+// answer is a prefix sum, so that nothing depends on the order of blocks or atomics.
+#include "sb_cache.cuh"
+
+namespace sb {
+
+namespace {
+
+constexpr int kThreads = 256;
+
+struct Sums {
+    long long need, back, grow, parts;  // pages taken, pages given back, new tokens, pieces
+};
+__device__ inline Sums operator+(const Sums& a, const Sums& b) { return Sums{a.need + b.need, a.back + b.back, a.grow + b.grow, a.parts + b.parts}; }
+__device__ inline long long shfl_up64(long long x, int off) { return __shfl_up_sync(0xffffffffu, x, off); }
+
+// index of the range of `first` (n + 1 ascending starts) that holds i
+__device__ inline int range_of(const int* first, int n, int i) {
+    int lo = 0, hi = n - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (first[mid] <= i) lo = mid; else hi = mid - 1;
+    }
+    return lo;
+}
+
+// Every block computes the prefix sums over all requests for itself (a few KB from the L2; with it no block waits for another and one
+// launch does) and writes its share of the outputs.
+__global__ void __launch_bounds__(kThreads) blocks_kernel(const SbBlocksParams p) {
+    extern __shared__ int sh[];
+    const int R = p.requests, P = p.page_tokens, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int* const before = sh;                 // tokens before the step, [R]
+    int* const need = before + R;           // first page taken, [R + 1]
+    int* const back = need + R + 1;         // first page given back
+    int* const grow = back + R + 1;         // first new token
+    int* const parts = grow + R + 1;        // first piece
+    __shared__ Sums warp_sums[kThreads / 32];
+    __shared__ int bad_any;
+    if (threadIdx.x == 0) bad_any = 0;
+    pdl_wait();
+    pdl_launch_dependents();
+    __syncthreads();
+    const long long cap = (long long)p.width * P;
+    Sums carry{0, 0, 0, 0};
+    for (int base = 0; base < R; base += kThreads) {
+        const int r = base + threadIdx.x;
+        Sums mine{0, 0, 0, 0};
+        if (r < R) {
+            const long long len = p.lengths[r], n = p.new_tokens[r], after = len + n;
+            before[r] = (int)len;
+            if (len < 0 || len > cap || after < 0 || after > cap) {
+                bad_any = 1;
+            } else {
+                const long long had = (len + P - 1) / P, has = (after + P - 1) / P;
+                mine.need = has > had ? has - had : 0;
+                mine.back = had > has ? had - has : 0;
+                mine.grow = n > 0 ? n : 0;
+                mine.parts = n > 0 ? has - len / P : 0;
+            }
+        }
+        Sums x = mine;
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) {
+            const Sums y{shfl_up64(x.need, off), shfl_up64(x.back, off), shfl_up64(x.grow, off), shfl_up64(x.parts, off)};
+            if (lane >= off) x = x + y;
+        }
+        if (lane == 31) warp_sums[warp] = x;
+        __syncthreads();
+        Sums total = carry;
+        for (int w = 0; w < kThreads / 32; ++w) {
+            if (w == warp) carry = total;
+            total = total + warp_sums[w];
+        }
+        if (r < R) {  // exclusive: what the requests before r take; meaningless numbers where the step is refused, and not used then
+            need[r] = (int)(carry.need + x.need - mine.need);
+            back[r] = (int)(carry.back + x.back - mine.back);
+            grow[r] = (int)(carry.grow + x.grow - mine.grow);
+            parts[r] = (int)(carry.parts + x.parts - mine.parts);
+        }
+        carry = total;
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) {
+        need[R] = (int)carry.need;
+        back[R] = (int)carry.back;
+        grow[R] = (int)carry.grow;
+        parts[R] = (int)carry.parts;
+    }
+    __syncthreads();
+    const long long count = p.free_count[0], after_count = count + carry.back - carry.need;
+    const bool bad = bad_any || carry.grow > p.tokens || carry.parts > p.n_pieces || count < 0 || count > p.pages || after_count > p.pages;
+    const bool none = !bad && after_count < 0;
+    const bool refused = bad || none;
+
+    const long long stride = (long long)gridDim.x * kThreads, at = (long long)blockIdx.x * kThreads + threadIdx.x;
+    if (at == 0) {
+        p.free_count_out[0] = refused ? (int)count : (int)after_count;
+        if (refused) atomicOr(p.status, bad ? SBATTN_ST_BAD_SEQLENS : SBATTN_ST_NO_PAGES);
+    }
+    for (long long r = at; r < R; r += stride) {
+        p.lengths_out[r] = refused ? before[r] : before[r] + p.new_tokens[r];
+        p.ends[r] = refused ? 0 : grow[r + 1];
+    }
+    if (refused) {
+        for (long long t = at; t < p.tokens; t += stride) p.slots[t] = -1;
+        for (long long i = at; i < p.n_pieces; i += stride) ((int4*)p.pieces)[i] = make_int4(-1, 0, 0, 0);
+        return;
+    }
+    // page j of those given back, request by request in the order of their blocks
+    const auto given = [&](int j) {
+        const int r = range_of(back, R, j);
+        const int has = (before[r] + p.new_tokens[r] + P - 1) / P;
+        return p.tables[r * p.table_stride + has + (j - back[r])];
+    };
+    // page k of those taken: from the top of the stack, on which those given back lie first
+    const int top = (int)count + back[R] - 1;
+    const auto taken = [&](int k) { return top - k < (int)count ? p.free_pages[top - k] : given(top - k - (int)count); };
+    for (long long k = at; k < need[R]; k += stride) {
+        const int r = range_of(need, R, (int)k);
+        p.tables[r * p.table_stride + (before[r] + P - 1) / P + (k - need[r])] = taken((int)k);
+    }
+    for (long long j = at; j < after_count - count; j += stride) p.free_pages[count + j] = given((int)j);
+    const auto page_at = [&](int r, int block) {  // of a growing request, with the pages of this step
+        const int had = (before[r] + P - 1) / P;
+        return block < had ? p.tables[r * p.table_stride + block] : taken(need[r] + block - had);
+    };
+    for (long long t = at; t < p.tokens; t += stride) {
+        int slot = -1;
+        if (t < grow[R]) {
+            const int r = range_of(grow, R, (int)t), pos = before[r] + (int)t - grow[r];
+            const long long s = (long long)page_at(r, pos / P) * P + pos % P;
+            if (s >= 0 && s <= 0x7fffffffll) slot = (int)s;
+            else atomicOr(p.status, SBATTN_ST_BAD_PAGES);
+        }
+        p.slots[t] = slot;
+    }
+    for (long long i = at; i < p.n_pieces; i += stride) {
+        int4 piece = make_int4(-1, 0, 0, 0);
+        if (i < parts[R]) {
+            const int r = range_of(parts, R, (int)i), block = before[r] / P + (int)i - parts[r], start = block * P;
+            const int old = max(0, before[r] - start), stop = min(P, before[r] + p.new_tokens[r] - start);
+            piece = make_int4(page_at(r, block), grow[r] + max(0, start - before[r]), old, stop - old);
+        }
+        ((int4*)p.pieces)[i] = piece;
+    }
+}
+
+}  // namespace
+
+int launch_cache_blocks(const SbBlocksParams& p, cudaStream_t st) {
+    const size_t smem = sizeof(int) * ((size_t)p.requests * 5 + 4);
+    const int rc = ensure_kernel_attrs((const void*)blocks_kernel, (int)(sizeof(int) * (SBATTN_MAX_REQUESTS * 5 + 4)), false);
+    if (rc != 0) return rc;
+    const int64_t items = (int64_t)p.tokens + p.n_pieces + p.requests;
+    int64_t grid = (items + 4 * kThreads - 1) / (4 * kThreads);
+    if (grid > sm_count()) grid = sm_count();
+    if (grid < 1) grid = 1;
+    return launch_kernel(blocks_kernel, dim3((unsigned)grid), dim3(kThreads), smem, st, p);
+}
+
+}  // namespace sb

@@ -63,7 +63,9 @@ void maybe_check_status(int device) {
     const int v = w.item<int>();
     w.zero_();
     TORCH_CHECK_VALUE(!(v & SBATTN_ST_BAD_SEQLENS), "cu_seqlens rejected on the device: ends must be non-decreasing, at most the number of "
-                      "tokens, and no sequence longer than max_seqlens");
+                      "tokens, and no sequence longer than max_seqlens (cache: lengths within their tables, new tokens within them)");
+    TORCH_CHECK_VALUE(!(v & SBATTN_ST_BAD_PAGES), "a page index lies outside the cache, or the pieces do not fit it");
+    TORCH_CHECK_VALUE(!(v & SBATTN_ST_NO_PAGES), "the cache has fewer free pages than the new tokens need (nothing was added)");
     TORCH_CHECK(!(v & SBATTN_ST_TIMEOUT), "a stick-breaking attention kernel gave up waiting (results are invalid)");
 }
 
@@ -378,6 +380,186 @@ std::array<Tensor, 3> bwd(const Tensor& d_o, const Tensor& d_rem, const Tensor& 
     return backward(d_o, d_rem, q, k, v, cu, ws, rem ? *rem : Tensor(), Opts{batched, *max_seqlens, scale, attend_current, fused, path}, phases, out, bwd_ws);
 }
 
+// ------------------------------------------------------------------------------------------------------------ 8-bit paged cache
+void check_ints(const Tensor& t, const char* name, int ndim, const Tensor& like) {
+    TORCH_CHECK_TYPE(t.scalar_type() == at::kInt, name, " must be int32");
+    TORCH_CHECK_VALUE(t.dim() == ndim, name, " must be ", ndim, "-d");
+    TORCH_CHECK_VALUE(t.device() == like.device(), name, " must live on the device of the other tensors");
+}
+
+// (lengths, free_count, ends, slots, pieces) after the step; tables and free_pages are written in place
+std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> cache_blocks(const Tensor& lengths, const Tensor& new_tokens, const Tensor& tables, const Tensor& free_pages,
+                                                                const Tensor& free_count, int64_t page_tokens, int64_t tokens) {
+    TORCH_CHECK(lengths.is_cuda(), "the cache lives on CUDA tensors only (there is no CPU implementation)");
+    check_ints(lengths, "lengths", 1, lengths);
+    check_ints(new_tokens, "new_tokens", 1, lengths);
+    check_ints(tables, "tables", 2, lengths);
+    check_ints(free_pages, "free_pages", 1, lengths);
+    check_ints(free_count, "free_count", 1, lengths);
+    const int64_t R = lengths.size(0);
+    TORCH_CHECK_VALUE(new_tokens.size(0) == R && tables.size(0) == R, "lengths, new_tokens and tables must have one entry per request");
+    TORCH_CHECK_VALUE(free_count.size(0) == 1, "free_count must have one entry");
+    TORCH_CHECK_VALUE(tables.size(1) < 2 || tables.stride(1) == 1, "the rows of tables must be contiguous");
+    TORCH_CHECK_VALUE(free_pages.size(0) < 2 || free_pages.stride(0) == 1, "free_pages must be contiguous");
+    TORCH_CHECK_VALUE(R < 2 || tables.stride(0) >= tables.size(1), "the rows of tables must not overlap");
+    TORCH_CHECK_VALUE(page_tokens == 16 || page_tokens == 32 || page_tokens == 64 || page_tokens == 128, "page_tokens must be 16, 32, 64 or 128");
+    TORCH_CHECK_VALUE(tokens >= 0 && tokens <= (1 << 30), "tokens must be between 0 and 2^30");
+    TORCH_CHECK_VALUE(R <= SBATTN_MAX_REQUESTS, "more than ", SBATTN_MAX_REQUESTS, " requests");
+    TORCH_CHECK_VALUE(tables.size(1) * page_tokens <= (1 << 30) && free_pages.size(0) <= 0x7fffffff, "tables of more than 2^30 tokens per request");
+    c10::cuda::OptionalCUDAGuard guard(lengths.device());
+    const Tensor len = lengths.contiguous(), more = new_tokens.contiguous();
+    const int64_t n_pieces = sbattn_cache_pieces(R, tokens, page_tokens);
+    const auto ints = [&](at::IntArrayRef s) { return empty_like_dtype(len, s, at::kInt); };
+    const Tensor pieces = ints({n_pieces, 4}), after = ints({R}), count = ints({1}), ends = ints({R}), slots = ints({tokens});
+    SbBlocksParams p{};
+    p.requests = (int32_t)R;
+    p.width = (int32_t)tables.size(1);
+    p.pages = (int32_t)free_pages.size(0);
+    p.page_tokens = (int32_t)page_tokens;
+    p.tokens = (int32_t)tokens;
+    p.n_pieces = (int32_t)n_pieces;
+    p.table_stride = std::max(tables.stride(0), tables.size(1));
+    p.lengths = len.const_data_ptr<int32_t>();
+    p.new_tokens = more.const_data_ptr<int32_t>();
+    p.free_count = free_count.const_data_ptr<int32_t>();
+    p.tables = tables.data_ptr<int32_t>();
+    p.free_pages = free_pages.data_ptr<int32_t>();
+    p.lengths_out = after.data_ptr<int32_t>();
+    p.free_count_out = count.data_ptr<int32_t>();
+    p.ends = ends.data_ptr<int32_t>();
+    p.slots = slots.data_ptr<int32_t>();
+    p.pieces = pieces.data_ptr<int32_t>();
+    p.status = status_ptr(len.get_device());
+    p.stream = c10::cuda::getCurrentCUDAStream(len.get_device()).stream();
+    check(sbattn_cache_blocks(&p), "sbattn_cache_blocks");
+    maybe_check_status(len.get_device());
+    return {after, count, ends, slots, pieces};
+}
+
+// the four tensors of a cache into p; head_dim is that of the caller's keys or queries
+void cache_into(SbCacheParams& p, const Tensor& kc, const Tensor& vc, const Tensor& ks, const Tensor& vs, const Tensor& x) {
+    TORCH_CHECK(x.is_cuda(), "stick-breaking attention runs on CUDA tensors only (there is no CPU implementation)");
+    TORCH_CHECK_VALUE(x.dim() == 3, "q, k and v are [heads, tokens, head_dim]");
+    p.dtype = dtype_of(x);
+    TORCH_CHECK_TYPE(kc.scalar_type() == at::kFloat8_e4m3fn && vc.scalar_type() == at::kFloat8_e4m3fn, "the codes of a cache are float8_e4m3fn");
+    TORCH_CHECK_TYPE(ks.scalar_type() == at::kFloat && vs.scalar_type() == at::kFloat, "the scales of a cache are float32");
+    TORCH_CHECK_VALUE(kc.dim() == 4 && vc.sizes() == kc.sizes(), "the codes of a cache are [pages, heads, page_tokens, row], for keys and values alike");
+    TORCH_CHECK_VALUE(ks.dim() == 2 && vs.sizes() == ks.sizes() && ks.size(0) == kc.size(0) && ks.size(1) == kc.size(1), "the scales of a cache are [pages, heads]");
+    for (const Tensor* t : {&kc, &vc, &ks, &vs}) TORCH_CHECK_VALUE(t->device() == x.device(), "the cache must live on the device of q, k and v");
+    const int64_t D = x.size(2), row = D <= 32 ? 32 : D <= 64 ? 64 : 128, P = kc.size(2);
+    TORCH_CHECK_VALUE(D >= 1 && D <= 128, "head_dim must be between 1 and 128");
+    TORCH_CHECK_VALUE(kc.size(3) == row, "the rows of this cache have ", kc.size(3), " places, those of head_dim ", D, " need ", row);
+    TORCH_CHECK_VALUE(P == 16 || P == 32 || P == 64 || P == 128, "a page holds 16, 32, 64 or 128 tokens");
+    TORCH_CHECK_VALUE(kc.size(0) >= 1 && kc.size(0) <= 0x7fffffff && kc.size(1) <= 65535, "a cache has at least one page and at most 65535 heads");
+    TORCH_CHECK_VALUE(x.size(0) <= 65535 && x.size(1) <= (1 << 30), "too many heads or tokens");
+    const auto pages = [&](const Tensor& t) {
+        TORCH_CHECK_VALUE(t.stride(3) == 1 && t.stride(2) == row && (t.size(1) < 2 || t.stride(1) == P * row), "the codes of a page must be contiguous");
+        TORCH_CHECK_VALUE(t.size(0) < 2 || t.stride(0) >= t.size(1) * P * row, "the pages of a cache must not overlap");
+        return t.size(0) < 2 ? t.size(1) * P * row : t.stride(0);
+    };
+    const auto scales = [&](const Tensor& t) {
+        TORCH_CHECK_VALUE((t.size(1) < 2 || t.stride(1) == 1) && (t.size(0) < 2 || t.stride(0) >= t.size(1)), "the scales of a page must be contiguous");
+        return t.size(0) < 2 ? t.size(1) : t.stride(0);
+    };
+    p.kv_heads = (int32_t)kc.size(1);
+    p.head_dim = (int32_t)D;
+    p.row = (int32_t)row;
+    p.page_tokens = (int32_t)P;
+    p.pages = (int32_t)kc.size(0);
+    p.tokens = (int32_t)x.size(1);
+    p.k_stride = pages(kc);
+    p.v_stride = pages(vc);
+    p.k_scale_stride = scales(ks);
+    p.v_scale_stride = scales(vs);
+    p.k_codes = kc.data_ptr();
+    p.v_codes = vc.data_ptr();
+    p.k_scale = ks.data_ptr<float>();
+    p.v_scale = vs.data_ptr<float>();
+    p.status = status_ptr(x.get_device());
+    p.stream = c10::cuda::getCurrentCUDAStream(x.get_device()).stream();
+}
+
+void cache_append(const Tensor& k, const Tensor& v, const Tensor& kc, const Tensor& vc, const Tensor& ks, const Tensor& vs, const Tensor& pieces) {
+    at::NoGradGuard no_grad;
+    SbCacheParams p{};
+    c10::cuda::OptionalCUDAGuard guard(k.device());
+    cache_into(p, kc, vc, ks, vs, k);
+    TORCH_CHECK_VALUE(v.sizes() == k.sizes(), "k and v must share one shape");
+    TORCH_CHECK_TYPE(v.scalar_type() == k.scalar_type(), "k and v must share one dtype");
+    TORCH_CHECK_VALUE(v.device() == k.device(), "k and v must live on one device");
+    TORCH_CHECK_VALUE(k.size(0) == kc.size(1), "k and v have ", k.size(0), " heads, the cache has ", kc.size(1));
+    check_ints(pieces, "pieces", 2, k);
+    TORCH_CHECK_VALUE(pieces.size(1) == 4 && pieces.is_contiguous(), "pieces is a contiguous [n, 4] tensor of sb_cache_blocks");
+    const Tensor kk = unit_inner(k), vv = unit_inner(v);
+    p.n_pieces = (int32_t)pieces.size(0);
+    p.pieces = pieces.const_data_ptr<int32_t>();
+    p.k = mat(kk, false);
+    p.v = mat(vv, false);
+    check(sbattn_cache_append(&p), "sbattn_cache_append");
+    maybe_check_status(k.get_device());
+}
+
+std::pair<Tensor, Tensor> attend_cached(const Tensor& q_, const Tensor& kc, const Tensor& vc, const Tensor& ks, const Tensor& vs, const Tensor& tables, const Tensor& lengths,
+                                        const OptTensor& ends_, double scale, bool attend_current, const OptTensor& v_) {
+    SbCacheParams p{};
+    TORCH_CHECK(!(at::GradMode::is_enabled() && (q_.requires_grad() || (v_ && v_->requires_grad()))),
+                "attention over the cache has no backward: call it under torch.no_grad() or with tensors that need no gradient");
+    TORCH_CHECK_NOT_IMPLEMENTED(!q_._fw_grad(0).defined() && !(v_ && v_->_fw_grad(0).defined()), "stick-breaking attention does not implement forward mode AD");
+    at::NoGradGuard no_grad;
+    c10::cuda::OptionalCUDAGuard guard(q_.device());
+    cache_into(p, kc, vc, ks, vs, q_);
+    const Tensor q = unit_inner(q_);
+    const int64_t R = lengths.numel();
+    TORCH_CHECK_VALUE(kc.size(1) > 0 ? q.size(0) % kc.size(1) == 0 : q.size(0) == 0, "the heads of q must be a multiple of the cache's");
+    check_ints(lengths, "lengths", 1, q);
+    check_ints(tables, "tables", 2, q);
+    TORCH_CHECK_VALUE(tables.size(0) == R, "lengths and tables must have one entry per request");
+    TORCH_CHECK_VALUE(R <= SBATTN_MAX_REQUESTS, "more than ", SBATTN_MAX_REQUESTS, " requests");
+    TORCH_CHECK_VALUE(tables.size(1) < 2 || tables.stride(1) == 1, "the rows of tables must be contiguous");
+    TORCH_CHECK_VALUE(tables.size(1) * kc.size(2) <= (1 << 30), "tables of more than 2^30 tokens per request");
+    const Tensor len = lengths.contiguous();
+    const Tensor tab = R < 2 || tables.stride(0) >= tables.size(1) ? tables : tables.contiguous();  // one row for all requests: a copy
+    Tensor ends, v;
+    if (ends_) {
+        check_ints(*ends_, "ends", 1, q);
+        TORCH_CHECK_VALUE(ends_->size(0) == R, "ends must have one entry per request");
+        ends = ends_->contiguous();
+        p.ends = ends.const_data_ptr<int32_t>();
+    } else {
+        TORCH_CHECK_VALUE(q.size(1) >= R, "without ends, q has a row for every request");
+    }
+    if (v_) {
+        TORCH_CHECK_TYPE(v_->scalar_type() == q.scalar_type(), "q and v must share one dtype");
+        TORCH_CHECK_VALUE(v_->dim() == 3 && v_->size(0) == kc.size(1) && v_->size(1) == q.size(1) && v_->size(2) == q.size(2) && v_->device() == q.device(),
+                          "v must be [heads of the cache, tokens of q, head_dim], on the device of q");
+        v = unit_inner(*v_);
+        p.v = mat(v, false);
+    }
+    const Tensor o = empty_rows(q), rem = empty_like_dtype(q, q.sizes().slice(0, 2), q.scalar_type());
+    p.heads = (int32_t)q.size(0);
+    p.requests = (int32_t)R;
+    p.width = (int32_t)tab.size(1);
+    p.attend_current = attend_current;
+    p.inv_temp = (float)scale;
+    p.q = mat(q, false);
+    p.o = mat(o, false);
+    p.rem = vec(rem, false);
+    p.tables = tab.const_data_ptr<int32_t>();
+    p.table_stride = std::max(tab.stride(0), tab.size(1));
+    p.lengths = len.const_data_ptr<int32_t>();
+    size_t need = 0;
+    check(sbattn_cached_workspace_bytes(&p, &need), "sbattn_cached_workspace_bytes");
+    Tensor ws;
+    if (need > 0) {
+        ws = bytes(need, q);
+        p.workspace = ws.data_ptr();
+        p.workspace_bytes = need;
+    }
+    check(sbattn_cached_fwd(&p), "sbattn_cached_fwd");
+    maybe_check_status(q.get_device());
+    return {o, rem};
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_binding, m) {
@@ -405,4 +587,7 @@ PYBIND11_MODULE(_binding, m) {
     m.def("bwd", &bwd, unlocked);
     m.def("seq_bounds", &seq_bounds, unlocked);
     m.def("status_word", &status_word, unlocked);
+    m.def("cache_blocks", &cache_blocks, unlocked);
+    m.def("cache_append", &cache_append, unlocked);
+    m.def("attend_cached", &attend_cached, unlocked);
 }

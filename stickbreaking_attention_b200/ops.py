@@ -69,7 +69,11 @@ def check_status(device=None, reset=True):
         w.zero_()
     if val & _lib.ST_BAD_SEQLENS:
         raise ValueError("cu_seqlens rejected on the device: ends must be non-decreasing, at most the number of "
-                         "tokens, and no sequence longer than max_seqlens")
+                         "tokens, and no sequence longer than max_seqlens (cache: lengths within their tables, new tokens within them)")
+    if val & _lib.ST_BAD_PAGES:
+        raise ValueError("a page index lies outside the cache, or the pieces do not fit it")
+    if val & _lib.ST_NO_PAGES:
+        raise ValueError("the cache has fewer free pages than the new tokens need (nothing was added)")
     if val & _lib.ST_TIMEOUT:
         raise RuntimeError("a stick-breaking attention kernel gave up waiting (results are invalid)")
     return val
