@@ -67,6 +67,7 @@ static int check_cached(const SbCacheParams* p) {
     if (p->heads < 0 || p->requests < 0 || p->width < 0) return SBATTN_EINVAL;
     if (p->kv_heads > 0 ? p->heads % p->kv_heads != 0 : p->heads != 0) return SBATTN_EINVAL;
     if (p->requests > SBATTN_MAX_REQUESTS || p->heads > 65535 || (int64_t)p->width * p->page_tokens > (1 << 30)) return SBATTN_EUNSUPPORTED;
+    if (p->kv_heads > 0 && (int64_t)p->tokens * (p->heads / p->kv_heads) > (1ll << 30)) return SBATTN_EUNSUPPORTED;
     return SBATTN_OK;
 }
 

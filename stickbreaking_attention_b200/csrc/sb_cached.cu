@@ -1,117 +1,693 @@
 // Stick-breaking attention of new tokens over the 8-bit paged cache.
+//
+// With s_ij = q_i . k_j * inv_temp, beta = 1 / (1 + exp(-s)) and soft(s) = log(1 + exp(s)) = -log(1 - beta), a query's weights are
+// A_ij = beta_ij exp(-sum of soft over the keys to the right of j that it sees), and two ranges of keys, each treated as if nothing were to its
+// right, join by o = o_right + exp(-S_right) o_left, S = S_right + S_left: no maximum and no renormalisation.  So the keys of all
+// requests and heads are one line of work, cut into equal shares for all warps of the GPU wherever the cuts fall.
+//
+// What bounds it is the cache's bytes (2 row bytes per key and head, once), as long as few queries share a key.  A warp goes through its share 32
+// keys at a time, from the right:
+//   * TMA loads of whole rows into a ring of its own, stages ahead; no barrier between warps;
+//   * codes become float16, exactly, on the way from shared memory to the operands of warp-level matrix instructions.  K is the left operand (16 keys)
+//     and the queries that share the keys (heads of a group, new tokens) are the 8 columns of the right one, V the left operand
+//     of the second product, d by keys.  Eight columns are what tcgen05's 128 rows would be filled with: the data path of 8-bit codes through the
+//     registers is needed either way, and the tensor pipe is idle most of the time;
+//   * a lane forms one key's weight for every column in float32: soft and its sums over the lanes by shuffles, the carry compensated;
+//   * the weights of 32 keys, with the scale of the values' page, are scaled by a power of two to at most 2^15 per column and split into two float16 terms
+//     (22 bits: what is lost is below float32's own rounding of the sums), the two products are added to float32 accumulators.
+// float32 queries are two float16 terms, too; 16-bit ones are scaled by a power of two per row and exact.
 #include "sb_cache.cuh"
+#include "sb_sm100.cuh"
 
 namespace sb {
 
 namespace {
 
-constexpr int kWarps = 4;
+using namespace sm100;
 
-// One warp per query row and head, 32 keys at a time from the right: a lane forms the score of one key, the suffix sums of log(1 - beta) go
-// over the lanes, and the weighted sum of the values is shared out by columns of D.
-template <typename T>
-__global__ void __launch_bounds__(32 * kWarps) cached_kernel(const SbCacheParams p) {
-    __shared__ float qs[kWarps][kMaxHeadDim], ws[kWarps][32];
-    __shared__ const uint8_t* vs[kWarps][32];
+constexpr int kWarps = 8, kThreads = 32 * kWarps;
+constexpr int kCols = 8;       // queries that share a key's product
+constexpr int kColStride = 40; // floats from column to column in the exchange buffer: 4-byte stores and 8-byte loads without bank conflicts
+
+__host__ __device__ constexpr int stages(int dp) { return dp == 32 ? 4 : 3; }
+__host__ __device__ constexpr int stage_bytes(int dp) { return 2 * 32 * dp; }
+
+struct WarpScratch {
+    float x[kCols * kColStride];  // scores, then the two terms of the weights
+    float carry[kCols], carry_low[kCols];  // sum of soft to the right of the present keys, and what rounding it has lost
+    float factor[kCols];          // power of two that the weights were divided by
+    float temp[kCols];            // inv_temp by what the query was multiplied with
+    float scale[4][4];            // per stage: keys' scale of the lower and upper 16 keys, values' scale
+    uint64_t full[4];
+};
+
+template <int DP>
+struct Layout {
+    static constexpr size_t ring = (size_t)kWarps * stages(DP) * stage_bytes(DP);
+    static constexpr size_t scratch = ring;
+    static constexpr size_t starts = scratch + kWarps * sizeof(WarpScratch);
+    static size_t bytes(int requests) { return 1024 + starts + sizeof(int) * ((size_t)requests + 1); }  // 1024: the ring is aligned by hand
+};
+__host__ __device__ constexpr int kSlot(int dp) { return kCols * dp + kCols; }  // floats of a partial result: [column][d], then the sums
+
+struct Job {
+    int r, g, tile;      // request, key/value head, tile of columns
+    int first, n, len;   // rows of q of the request, tokens
+    int pos, end, steps; // 32-key steps, counted from the right: [pos, end) of steps
+    int cols, keys;      // columns of the tile, keys that its last column sees
+};
+
+// What the host knows of a launch besides the parameters
+struct Plan {
+    int shared;          // queries' heads per key/value head
+    float* warp_slots;   // [grid * kWarps][2] partial results
+    float* block_slots;  // [grid][2]
+    int4* seams;         // [grid]: (request or -1, head, tile, last block) of the job that the block's first unit continues, if it started in the block before
+};
+
+__device__ __forceinline__ long long units_of(const Plan& pl, int len, int n, int see) {  // per key/value head
+    const int tiles = (n * pl.shared + kCols - 1) / kCols, keys = len - 1 + see;
+    return (long long)tiles * max(1, (keys + 31) >> 5);
+}
+
+__device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// four codes to two pairs of float16
+__device__ __forceinline__ void codes_to_f16(uint32_t w, uint32_t& lo, uint32_t& hi) {
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}" : "=r"(lo), "=r"(hi) : "r"(w));
+}
+__device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }  // -126 <= e <= 127
+
+// Places of rows in a stage.  Rows of 128 and 64 bytes are swizzled by TMA; which keys the lanes of a phase read is chosen so
+// that eight (16-byte loads) or sixteen of them (8-byte) meet all banks once.
+template <int DP> __device__ __forceinline__ int chunk_at(int key, int chunk) {
+    return DP == 128 ? key * 128 + ((chunk ^ (key & 7)) << 4) : key * 64 + ((chunk ^ ((key >> 1) & 3)) << 4);
+}
+template <int DP> __device__ __forceinline__ int key_of_row(int r) { return DP == 128 ? (r >> 1) | ((r & 1) << 2) : r; }
+template <int DP> __device__ __forceinline__ int key_of(int c, int i) {  // i-th of the four keys (of 16) of the lanes with lane % 4 = c
+    if (DP == 128) return 2 * c + (i & 1) + 8 * (i >> 1);
+    if (DP == 64) return (c & 1) + ((c >> 1) << 2) + 2 * (i & 1) + 8 * (i >> 1);
+    return c + 4 * i;
+}
+template <int DP> __device__ __forceinline__ int place_of(int key) {  // 16 * half + 4 c + i of a key (of 32)
+    const int k = key & 15;
+    if (DP == 128) return (key & 16) + 4 * ((k & 7) >> 1) + (k & 1) + 2 * (k >> 3);
+    if (DP == 64) return (key & 16) + 4 * ((k & 1) + ((k >> 1) & 2)) + ((k >> 1) & 1) + 2 * (k >> 3);
+    return (key & 16) + 4 * (k & 3) + (k >> 2);
+}
+
+template <typename T, int DP>
+struct Kernel {
+    static constexpr int ST = stages(DP), KW = DP / 16, VW = DP / 32, M = DP / 16;
+    static constexpr bool kSplitQ = sizeof(T) == 4;
+    const SbCacheParams& p;
+    const Plan& pl;
+    const int* starts;  // units per head before each request
+    int lane, see;
+
+    // the job of unit u, up to unit `stop`; r: a request at or before it
+    __device__ __forceinline__ Job open(long long u, long long stop, int r) const {
+        Job j;
+        while ((long long)starts[r + 1] * p.kv_heads <= u) ++r;
+        j.r = r;
+        request(r, j.first, j.n, j.len);
+        const int tiles = (j.n * pl.shared + kCols - 1) / kCols;
+        j.steps = max(1, (j.len - 1 + see + 31) >> 5);
+        const unsigned long long in = (unsigned long long)(u - (long long)starts[r] * p.kv_heads);
+        unsigned long long job;
+        if (in >> 32) {
+            job = in / (unsigned)j.steps;
+            j.pos = (int)(in % (unsigned)j.steps);
+        } else {
+            job = (unsigned)in / (unsigned)j.steps;
+            j.pos = (int)((unsigned)in % (unsigned)j.steps);
+        }
+        j.g = (int)(job / (unsigned)tiles);
+        j.tile = (int)(job % (unsigned)tiles);
+        j.end = (int)min((long long)j.steps, j.pos + (stop - u));
+        j.cols = min(kCols, j.n * pl.shared - j.tile * kCols);
+        j.keys = j.len - j.n + (j.tile * kCols + j.cols - 1) / pl.shared + see;
+        return j;
+    }
+    __device__ __forceinline__ void request(int r, int& first, int& n, int& len) const {
+        len = p.lengths[r];
+        if (p.ends) {
+            first = r > 0 ? p.ends[r - 1] : 0;
+            n = p.ends[r] - first;
+        } else {
+            first = r;
+            n = len > 0 ? 1 : 0;
+        }
+    }
+    // first step, counted from the right, that holds a key which the tile sees
+    __device__ __forceinline__ int first_pos(const Job& j) const { return max(j.pos, j.steps - max(1, (j.keys + 31) >> 5)); }
+    // keys that column c of the tile sees
+    __device__ __forceinline__ int sees(const Job& j, int c) const { return j.len - j.n + (j.tile * kCols + c) / pl.shared + see; }
+
+    __device__ __forceinline__ int row_of(const Job& j, int c, int& head) const {
+        const int col = j.tile * kCols + c;
+        head = j.g * pl.shared + col % pl.shared;
+        return j.first + col / pl.shared;
+    }
+    // results of one column: `n` values from d0 on, the sum of soft; `whole`: this thread writes rem
+    template <int N>
+    __device__ __forceinline__ void store(const Job& j, int c, int d0, const float (&x)[N], float sum, bool writes_rem) const {
+        int h;
+        const int t = row_of(j, c, h);
+        const T left = from_f32<T>(expf(-sum));
+        T* o = (T*)p.o.ptr + h * p.o.stride_h + t * p.o.stride_t;
+        const T* v = p.v.ptr ? (const T*)p.v.ptr + j.g * p.v.stride_h + t * p.v.stride_t : nullptr;
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (d0 + i < p.head_dim) o[d0 + i] = from_f32<T>(v ? fmaf(to_f32(left), to_f32(v[d0 + i]), x[i]) : x[i]);
+        if (writes_rem) ((T*)p.rem.ptr)[h * p.rem.stride_h + t * p.rem.stride_t] = left;
+    }
+};
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kThreads, DP == 128 ? 1 : 2)
+cached_kernel(const __grid_constant__ SbCacheParams p, const __grid_constant__ Plan pl, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
+    using K = Kernel<T, DP>;
+    constexpr int ST = K::ST, KW = K::KW, VW = K::VW, M = K::M;
+    extern __shared__ uint8_t raw[];
+    uint8_t* const sm = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);
+    __shared__ long long warp_sums[kWarps];
+    __shared__ uint32_t gave_up;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rr = lane >> 2, cc = lane & 3;
+    uint8_t* const ring = sm + (size_t)warp * ST * stage_bytes(DP);
+    WarpScratch& ws = ((WarpScratch*)(sm + Layout<DP>::scratch))[warp];
+    int* const starts = (int*)(sm + Layout<DP>::starts);
+    const int see = p.attend_current ? 1 : 0, P = p.page_tokens, R = p.requests;
+    if (lane == 0)
+        for (int s = 0; s < ST; ++s) mbar_init(&ws.full[s], 1);
+    if (threadIdx.x == 0) gave_up = 0;
+    fence_barrier_init();
     pdl_wait();
     pdl_launch_dependents();
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, h = blockIdx.y, t = blockIdx.x * kWarps + warp;
-    if (p.ends && blockIdx.x == 0 && blockIdx.y == 0)
-        for (int s = threadIdx.x; s < p.requests; s += 32 * kWarps)
-            if (p.ends[s] < (s > 0 ? p.ends[s - 1] : 0) || p.ends[s] > p.tokens) atomicOr(p.status, SBATTN_ST_BAD_SEQLENS);
-    if (t >= p.tokens) return;
-    const int D = p.head_dim, P = p.page_tokens, g = h / (p.heads / p.kv_heads);
-    int r = t, n = 1, i = 0;
-    if (p.ends) {
-        int lo = 0, hi = p.requests;
-        while (lo < hi) {
-            const int mid = (lo + hi) >> 1;
-            if (p.ends[mid] > t) hi = mid; else lo = mid + 1;
-        }
-        r = lo;
-        if (r < p.requests) {
-            const int first = r > 0 ? p.ends[r - 1] : 0;
-            n = p.ends[r] - first;
-            i = t - first;
-        }
-    }
-    T* rem = (T*)p.rem.ptr + h * p.rem.stride_h + t * p.rem.stride_t;
-    const int len = r < p.requests ? p.lengths[r] : 0;
-    if (r >= p.requests || (!p.ends && len == 0)) {
-        if (lane == 0) *rem = from_f32<T>(0.f);
-        return;
-    }
-    if (i < 0 || len < n || len > (int64_t)p.width * P) {
-        if (lane == 0) {
-            *rem = from_f32<T>(0.f);
-            atomicOr(p.status, SBATTN_ST_BAD_SEQLENS);
-        }
-        return;
-    }
-    const T* q = (const T*)p.q.ptr + h * p.q.stride_h + t * p.q.stride_t;
-    for (int d = lane; d < D; d += 32) qs[warp][d] = to_f32(q[d]);
-    const int keys = len - n + i + (p.attend_current ? 1 : 0);
-    float acc[4] = {0.f, 0.f, 0.f, 0.f}, right = 0.f;
-    for (int hi = keys; hi > 0; hi -= 32) {
-        const int j = hi - 1 - lane;
-        float x = 0.f, soft = 0.f, weight = 0.f;
-        const uint8_t* vp = nullptr;
-        __syncwarp();
-        if (j >= 0) {
-            int page = p.tables[r * p.table_stride + j / P];
-            if (page < 0 || page >= p.pages) {
-                atomicOr(p.status, SBATTN_ST_BAD_PAGES);
-                page = 0;
+
+    // where every request's units start: a prefix sum over the requests, by every block for itself
+    long long carry = 0;
+    bool bad = false;
+    for (int base = 0; base < R; base += kThreads) {
+        const int r = base + threadIdx.x;
+        long long mine = 0;
+        if (r < R) {
+            const int len = p.lengths[r];
+            int first = r, last = r + (len > 0 ? 1 : 0);
+            if (p.ends) {
+                first = r > 0 ? p.ends[r - 1] : 0;
+                last = p.ends[r];
             }
-            const int64_t at = ((int64_t)g * P + j % P) * p.row;
-            const uint8_t* kp = (const uint8_t*)p.k_codes + page * p.k_stride + at;
-            vp = (const uint8_t*)p.v_codes + page * p.v_stride + at;
-            for (int d = 0; d < D; ++d) x = fmaf(qs[warp][d], from_e4m3(kp[d]), x);
-            x *= p.k_scale[page * p.k_scale_stride + g] * p.inv_temp;
-            soft = fmaxf(x, 0.f) + log1pf(expf(-fabsf(x)));
-            if (x != x) soft = x;
-            weight = p.v_scale[page * p.v_scale_stride + g];
+            const long long n = (long long)last - first;
+            if (first < 0 || n < 0 || last > p.tokens || len < n || len > (long long)p.width * P) bad = true;
+            else if (n > 0) mine = units_of(pl, len, (int)n, see);
         }
-        float sum = soft;
+        long long x = mine;
 #pragma unroll
         for (int off = 1; off < 32; off <<= 1) {
-            const float y = __shfl_up_sync(0xffffffffu, sum, off);
-            if (lane >= off) sum += y;
+            const long long y = __shfl_up_sync(0xffffffffu, x, off);
+            if (lane >= off) x += y;
         }
-        const float before = __shfl_up_sync(0xffffffffu, sum, 1);  // the keys to the right of this one
-        weight *= expf(-(right + (lane > 0 ? before : 0.f))) / (1.f + expf(-x));
-        ws[warp][lane] = weight;
-        vs[warp][lane] = vp;
-        right += __shfl_sync(0xffffffffu, sum, 31);
-        __syncwarp();
-        for (int l = 0; l < 32 && l < hi; ++l) {
-            const float w = ws[warp][l];
-            for (int c = 0; c < 4; ++c)
-                if (lane + 32 * c < D) acc[c] = fmaf(w, from_e4m3(vs[warp][l][lane + 32 * c]), acc[c]);
+        if (lane == 31) warp_sums[warp] = x;
+        __syncthreads();
+        long long before = carry;
+        for (int w = 0; w < kWarps; ++w) {
+            if (w < warp) before += warp_sums[w];
+            carry += warp_sums[w];
+        }
+        if (r < R) starts[r] = (int)min(before + x - mine, 0x7fffffffll);
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) starts[R] = (int)min(carry, 0x7fffffffll);
+    if (carry > 0x7fffffffll) bad = true, carry = 0;
+    if (bad) atomicOr(p.status, SBATTN_ST_BAD_SEQLENS);
+    __syncthreads();
+    // rem of the rows that belong to no request
+    if (p.ends) {
+        const int first = R > 0 ? max(0, p.ends[R - 1]) : 0;
+        const long long rows = (long long)max(0, p.tokens - first) * p.heads;
+        for (long long i = (long long)blockIdx.x * kThreads + threadIdx.x; i < rows; i += (long long)gridDim.x * kThreads)
+            ((T*)p.rem.ptr)[(i % p.heads) * p.rem.stride_h + (first + i / p.heads) * p.rem.stride_t] = from_f32<T>(0.f);
+    } else {
+        for (long long i = (long long)blockIdx.x * kThreads + threadIdx.x; i < (long long)p.tokens * p.heads; i += (long long)gridDim.x * kThreads) {
+            const int t = (int)(i / p.heads);
+            if (t >= R || p.lengths[t] <= 0) ((T*)p.rem.ptr)[(i % p.heads) * p.rem.stride_h + t * p.rem.stride_t] = from_f32<T>(0.f);
         }
     }
-    const T left = from_f32<T>(expf(-right));
-    T* o = (T*)p.o.ptr + h * p.o.stride_h + t * p.o.stride_t;
-    const T* v = p.v.ptr ? (const T*)p.v.ptr + g * p.v.stride_h + t * p.v.stride_t : nullptr;
-    for (int c = 0; c < 4; ++c)
-        if (const int d = lane + 32 * c; d < D) o[d] = from_f32<T>(v ? fmaf(to_f32(left), to_f32(v[d]), acc[c]) : acc[c]);
-    if (lane == 0) *rem = left;
+
+    const long long units = carry * p.kv_heads;
+    // blocks with work, each with a unit per warp at least where there are so many
+    const long long active = max(1ll, min((long long)gridDim.x, units / kWarps));
+    const long long b0 = min(units, units * blockIdx.x / active), b1 = min(units, units * (blockIdx.x + 1) / active);
+    const long long w0 = b0 + (b1 - b0) * warp / kWarps, w1 = b0 + (b1 - b0) * (warp + 1) / kWarps;
+    const K k{p, pl, starts, lane, see};
+    int r0 = 0;  // the last request whose units start at or before w0
+    {
+        int hi = R;
+        while (hi - r0 > 1) {
+            const int mid = (r0 + hi) >> 1;
+            if ((long long)starts[mid] * p.kv_heads <= w0) r0 = mid; else hi = mid;
+        }
+    }
+
+    // ---- loads: unit iu is the next one; lane l holds the pages and scales of the l-th step of a batch of 32
+    long long iu = w0;
+    Job ij;
+    ij.r = r0;
+    int istage = 0, ipos = 0, ibatch = 0, iend = 0;
+    int page0 = 0, page1 = 0;
+    float4 sc = make_float4(0.f, 0.f, 0.f, 0.f);
+    const int box = min(32, P);
+    const auto issue = [&]() {
+        while (ipos >= iend) {  // the next job with steps of its own in this warp's share
+            if (iu >= w1) return;
+            ij = k.open(iu, w1, ij.r);
+            iu += ij.end - ij.pos;
+            ipos = k.first_pos(ij);
+            iend = ij.end;
+            ibatch = ipos;
+        }
+        if (ipos == ibatch) {
+            const int key = 32 * (ij.steps - 1 - (ipos + lane));  // first key of this lane's step
+            page0 = page1 = 0;
+            sc = make_float4(0.f, 0.f, 0.f, 0.f);
+            bool wrong = false;
+            if (ipos + lane < iend) {
+                const int* table = p.tables + ij.r * p.table_stride;
+                const auto look = [&](int at, float& ks, float& vs) {
+                    int page = table[at / P];
+                    if (page < 0 || page >= p.pages) {
+                        wrong = true;
+                        page = 0;
+                    }
+                    ks = p.k_scale[page * p.k_scale_stride + ij.g];
+                    vs = p.v_scale[page * p.v_scale_stride + ij.g];
+                    return page;
+                };
+                if (key < ij.keys) page0 = look(key, sc.x, sc.z);
+                sc.y = sc.x;
+                sc.w = sc.z;
+                page1 = page0;
+                if (P == 16 && key + 16 < ij.keys) page1 = look(key + 16, sc.y, sc.w);
+            }
+            if (wrong) atomicOr(p.status, SBATTN_ST_BAD_PAGES);
+            ibatch += 32;
+        }
+        if (lane == ((ipos - (ibatch - 32)) & 31)) {
+            const int key = 32 * (ij.steps - 1 - ipos), row = ij.g * P + key % P;
+            uint8_t* const dst = ring + istage * stage_bytes(DP);
+            const bool load = key < ij.keys, two = P == 16 && key + 16 < ij.keys;
+            *(float4*)ws.scale[istage] = sc;
+            mbar_expect_tx(&ws.full[istage], (load ? 2 * box * DP : 0) + (two ? 2 * box * DP : 0));
+            if (load) {
+                tma_load_3d(dst, &kmap, &ws.full[istage], 0, row, page0);
+                tma_load_3d(dst + 32 * DP, &vmap, &ws.full[istage], 0, row, page0);
+            }
+            if (two) {
+                tma_load_3d(dst + 16 * DP, &kmap, &ws.full[istage], 0, row, page1);
+                tma_load_3d(dst + 48 * DP, &vmap, &ws.full[istage], 0, row, page1);
+            }
+        }
+        ++ipos;
+        if (++istage == ST) istage = 0;
+    };
+    if (w0 < w1)
+        for (int s = 0; s < ST; ++s) issue();
+
+    // ---- steps
+    int stage = 0;
+    uint32_t parity = 0;
+    bool alive = true;
+    const int pk = key_of_row<DP>(rr);
+    Job j;
+    j.r = r0;
+    for (long long u = w0; u < w1 && alive;) {
+        j = k.open(u, w1, j.r);
+        const bool starts_here = j.pos == 0, ends_here = j.end == j.steps;
+        u += j.end - j.pos;
+        const int least = k.sees(j, 0);  // keys that every column sees
+
+        // the queries: column rr, the d's of this lane's words, scaled to at most 2^15
+        uint32_t qh[2 * KW], ql[K::kSplitQ ? 2 * KW : 1];
+        {
+            float x[4 * KW];
+            float top = 0.f;
+            int h = 0, t = 0;
+            if (rr < j.cols) t = k.row_of(j, rr, h);
+            const T* q = (const T*)p.q.ptr + h * p.q.stride_h + t * p.q.stride_t;
+#pragma unroll
+            for (int w = 0; w < KW; ++w) {
+                const int d = DP == 128 ? 16 * (cc + 4 * (w >> 2)) + 4 * (w & 3) : DP == 64 ? 16 * cc + 4 * w : 8 * cc + 4 * w;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    x[4 * w + i] = rr < j.cols && d + i < p.head_dim ? to_f32(q[d + i]) : 0.f;
+                    const float a = fabsf(x[4 * w + i]);
+                    if (a <= 3.4028234664e38f) top = fmaxf(top, a);
+                }
+            }
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            const int e = top > 0.f ? max((int)(__float_as_uint(top) >> 23) - 127, -112) : 14;  // up to 2^(e + 1)
+            const float up = pow2(14 - e);
+#pragma unroll
+            for (int i = 0; i < 2 * KW; ++i) {
+                const float a = x[2 * i] * up, b = x[2 * i + 1] * up;
+                qh[i] = pack_f16(a, b);
+                if (K::kSplitQ) {
+                    const __half2 hi = *(const __half2*)&qh[i];
+                    const float la = a - __low2float(hi), lb = b - __high2float(hi);  // NaN behind an infinity: the low term of that is zero
+                    ql[i] = pack_f16(fabsf(a) <= 65504.f ? la : 0.f, fabsf(b) <= 65504.f ? lb : 0.f);
+                }
+            }
+            __syncwarp();
+            if (cc == 0) {
+                ws.temp[rr] = p.inv_temp * pow2(e - 14);
+                ws.carry[rr] = ws.carry_low[rr] = 0.f;
+            }
+            __syncwarp();
+        }
+        float acc[M][4];
+#pragma unroll
+        for (int m = 0; m < M; ++m) acc[m][0] = acc[m][1] = acc[m][2] = acc[m][3] = 0.f;
+
+        for (int pos = k.first_pos(j); pos < j.end; ++pos) {
+            const int key0 = 32 * (j.steps - 1 - pos);
+            if (!mbar_wait(&ws.full[stage], parity, &gave_up)) {
+                alive = false;
+                break;
+            }
+            const uint8_t* const kt = ring + stage * stage_bytes(DP);
+            const uint8_t* const vt = kt + 32 * DP;
+            // scores: 2 x 16 keys by 8 columns
+#pragma unroll
+            for (int mt = 0; mt < 2; ++mt) {
+                float s[4] = {0.f, 0.f, 0.f, 0.f};
+                const int ka = 16 * mt + pk, kb = ka + 8;
+                uint32_t wa[KW], wb[KW];
+                if constexpr (DP == 32) {
+                    *(uint2*)wa = *(const uint2*)(kt + ka * 32 + cc * 8);
+                    *(uint2*)wb = *(const uint2*)(kt + kb * 32 + cc * 8);
+                } else {
+#pragma unroll
+                    for (int x = 0; x < KW / 4; ++x) {
+                        *(uint4*)(wa + 4 * x) = *(const uint4*)(kt + chunk_at<DP>(ka, cc + 4 * x));
+                        *(uint4*)(wb + 4 * x) = *(const uint4*)(kt + chunk_at<DP>(kb, cc + 4 * x));
+                    }
+                }
+#pragma unroll
+                for (int w = 0; w < KW; ++w) {
+                    uint32_t a0, a1, a2, a3;
+                    codes_to_f16(wa[w], a0, a2);
+                    codes_to_f16(wb[w], a1, a3);
+                    mma16816(s, a0, a1, a2, a3, qh[2 * w], qh[2 * w + 1]);
+                    if (K::kSplitQ) mma16816(s, a0, a1, a2, a3, ql[2 * w], ql[2 * w + 1]);
+                }
+                float* const x0 = ws.x + 2 * cc * kColStride + ka;
+                x0[0] = s[0];
+                x0[kColStride] = s[1];
+                x0[8] = s[2];
+                x0[kColStride + 8] = s[3];
+            }
+            __syncwarp();
+            // weights: a lane has a key
+            const float ks = ws.scale[stage][lane >> 4], vs = ws.scale[stage][2 + (lane >> 4)];
+            const int place = place_of<DP>(lane);
+            for (int c = 0; c < j.cols; ++c) {
+                float* const col = ws.x + c * kColStride;
+                const bool seen = key0 + lane < k.sees(j, c);
+                const float x = col[lane] * (ws.temp[c] * ks);
+                const float e = expf(-fabsf(x));
+                float soft = fmaxf(x, 0.f) + log1pf(e);
+                if (x != x) soft = x;
+                float weight = __fdividef(x >= 0.f ? 1.f : e, 1.f + e);
+                if (!seen) soft = 0.f;
+                float sum = soft;
+#pragma unroll
+                for (int off = 1; off < 32; off <<= 1) {
+                    const float y = __shfl_down_sync(0xffffffffu, sum, off);
+                    if (lane + off < 32) sum += y;
+                }
+                float right = __shfl_down_sync(0xffffffffu, sum, 1);
+                if (lane == 31) right = 0.f;
+                const float total = __shfl_sync(0xffffffffu, sum, 0), had = ws.carry[c], low = ws.carry_low[c];
+                weight = seen ? weight * vs * expf(-(had + (low + right))) : 0.f;
+                // to at most 2^15, and in two terms
+                const int e2 = max((int)(__reduce_max_sync(0xffffffffu, __float_as_uint(weight) & 0x7fffffffu) >> 23), 15);
+                const float y = weight * pow2(14 + 127 - e2);
+                const __half hi = __float2half_rn(y);
+                const float rest = y - __half2float(hi);
+                const __half lo = __float2half_rn(fabsf(y) <= 65504.f ? rest : 0.f);
+                __syncwarp();
+                ((__half*)col)[place] = hi;
+                ((__half*)col)[32 + place] = lo;
+                if (lane == 0) {
+                    ws.factor[c] = pow2(e2 - 127 - 14);
+                    const float now = had + total, part = now - had;  // two-sum
+                    ws.carry_low[c] = now <= 3.4028234664e38f ? low + ((had - (now - part)) + (total - part)) : 0.f;
+                    ws.carry[c] = now;
+                }
+            }
+            __syncwarp();
+            // weights times values
+            const bool edge = key0 + 32 > least;
+            bool mixed_nan = false;
+            uint32_t vw[2][4][VW];
+#pragma unroll
+            for (int ks16 = 0; ks16 < 2; ++ks16)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int key = 16 * ks16 + key_of<DP>(cc, i);
+                    uint32_t(&w)[VW] = vw[ks16][i];
+                    if constexpr (DP == 128) *(uint4*)w = *(const uint4*)(vt + chunk_at<DP>(key, rr));
+                    else if constexpr (DP == 64) *(uint2*)w = *(const uint2*)(vt + chunk_at<DP>(key, rr >> 1) + 8 * (rr & 1));
+                    else w[0] = *(const uint32_t*)(vt + key * 32 + rr * 4);
+                    if (edge && key0 + key >= least) {  // keys that some columns do not see: 0 * NaN would be NaN
+#pragma unroll
+                        for (int x = 0; x < VW; ++x) {
+                            if (key0 + key >= j.keys) w[x] = 0;
+                            const uint32_t nan = (((w[x] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7;
+                            if (nan) mixed_nan = true;
+                            w[x] &= ~(nan * 255u);
+                        }
+                    }
+                }
+            const float f0 = ws.factor[2 * cc], f1 = ws.factor[2 * cc + 1];
+            uint32_t bh[2][2], bl[2][2];
+#pragma unroll
+            for (int ks16 = 0; ks16 < 2; ++ks16) {
+                const uint2 h = *(const uint2*)((const __half*)(ws.x + rr * kColStride) + 16 * ks16 + 4 * cc);
+                const uint2 l = *(const uint2*)((const __half*)(ws.x + rr * kColStride) + 32 + 16 * ks16 + 4 * cc);
+                bh[ks16][0] = h.x, bh[ks16][1] = h.y, bl[ks16][0] = l.x, bl[ks16][1] = l.y;
+            }
+#pragma unroll
+            for (int w = 0; w < VW; ++w) {
+                float t[2][4] = {};
+#pragma unroll
+                for (int ks16 = 0; ks16 < 2; ++ks16)
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        uint32_t a0, a1, a2, a3;
+                        codes_to_f16(__byte_perm(vw[ks16][0][w], vw[ks16][1][w], half ? 0x7362 : 0x5140), a0, a1);
+                        codes_to_f16(__byte_perm(vw[ks16][2][w], vw[ks16][3][w], half ? 0x7362 : 0x5140), a2, a3);
+                        mma16816(t[half], a0, a1, a2, a3, bh[ks16][0], bh[ks16][1]);
+                        mma16816(t[half], a0, a1, a2, a3, bl[ks16][0], bl[ks16][1]);
+                    }
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    float(&a)[4] = acc[2 * w + half];
+                    a[0] = fmaf(f0, t[half][0], a[0]);
+                    a[1] = fmaf(f1, t[half][1], a[1]);
+                    a[2] = fmaf(f0, t[half][2], a[2]);
+                    a[3] = fmaf(f1, t[half][3], a[3]);
+                }
+            }
+            if (edge && __any_sync(0xffffffffu, mixed_nan)) {  // NaN for the columns that do see them
+                for (int key = max(0, least - key0); key < min(32, j.keys - key0); ++key)
+#pragma unroll
+                    for (int m = 0; m < M; ++m)
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            const int d = rr * 4 * VW + 2 * m + i, at = DP == 32 ? key * 32 + d : chunk_at<DP>(key, d >> 4) + (d & 15);
+                            if ((vt[at] & 127) == 127)
+#pragma unroll
+                                for (int c = 0; c < 2; ++c)
+                                    if (key0 + key < k.sees(j, 2 * cc + c)) acc[m][2 * i + c] = __int_as_float(0x7fc00000);
+                        }
+            }
+            __syncwarp();
+            issue();
+            if (++stage == ST) {
+                stage = 0;
+                parity ^= 1;
+            }
+        }
+        if (!alive) break;
+        // the share's part of this job: the result, or a partial one
+        float* const slot = pl.warp_slots + ((size_t)(blockIdx.x * kWarps + warp) * 2 + (starts_here ? 1 : 0)) * kSlot(DP);
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            const int col = 2 * cc + c, d0 = rr * 4 * VW;
+            if (col >= j.cols) continue;
+            float x[2 * M];
+#pragma unroll
+            for (int m = 0; m < M; ++m) {
+                x[2 * m] = acc[m][c];
+                x[2 * m + 1] = acc[m][2 + c];
+            }
+            const float sum = ws.carry[col] + ws.carry_low[col];
+            if (starts_here && ends_here) {
+                k.store(j, col, d0, x, sum, rr == 0);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 2 * M; ++i) slot[col * DP + d0 + i] = x[i];
+                if (rr == 0) slot[kCols * DP + col] = sum;
+            }
+        }
+        __syncwarp();
+    }
+    if (!alive) {  // no load of this warp may arrive after it has left
+        uint32_t ignored = 0;
+        for (int s = 0; s < ST; ++s) {
+            mbar_wait(&ws.full[stage], parity, &ignored);
+            if (++stage == ST) {
+                stage = 0;
+                parity ^= 1;
+            }
+        }
+        if (lane == 0) atomicOr(p.status, SBATTN_ST_TIMEOUT);
+    }
+
+    // ---- jobs that several warps of this block share: joined by the warp that has their first part here
+    __syncthreads();
+    if (gave_up || b0 >= b1) {
+        if (threadIdx.x == 0) pl.seams[blockIdx.x] = make_int4(-1, 0, 0, 0);
+        return;
+    }
+    constexpr int N = DP / 32;
+    const auto join = [&](long long u) {  // the job of unit u, the first of its units in this warp's share
+        const Job j = k.open(u, b1, r0);
+        const long long first = u - j.pos, last = first + j.steps;  // the job's units
+        const bool from_before = first < b0, goes_on = last > b1;
+        for (int c = 0; c < j.cols; ++c) {
+            float x[N] = {}, sum = 0.f;
+            for (int w = warp; w < kWarps; ++w) {
+                const long long s0 = b0 + (b1 - b0) * w / kWarps, s1 = b0 + (b1 - b0) * (w + 1) / kWarps;
+                if (s0 >= last) break;
+                if (s0 == s1) continue;
+                const float* slot = pl.warp_slots + ((size_t)(blockIdx.x * kWarps + w) * 2 + (first >= s0 ? 1 : 0)) * kSlot(DP);
+                const float weight = expf(-sum);
+#pragma unroll
+                for (int i = 0; i < N; ++i) x[i] = fmaf(weight, slot[c * DP + lane * N + i], x[i]);
+                sum += slot[kCols * DP + c];
+            }
+            if (!from_before && !goes_on) {
+                k.store(j, c, lane * N, x, sum, lane == 0);
+            } else {
+                float* slot = pl.block_slots + ((size_t)blockIdx.x * 2 + (from_before ? 0 : 1)) * kSlot(DP);
+#pragma unroll
+                for (int i = 0; i < N; ++i) slot[c * DP + lane * N + i] = x[i];
+                if (lane == 0) slot[kCols * DP + c] = sum;
+            }
+        }
+        if (lane == 0 && from_before) {  // the join kernel's block of this seam takes the job if it started in the block before
+            const long long before = units * ((long long)blockIdx.x - 1) / active;
+            const int last_block = (int)((last * active - 1) / units);  // of unit last - 1
+            pl.seams[blockIdx.x] = first >= before ? make_int4(j.r, j.g, j.tile, last_block) : make_int4(-1, 0, 0, 0);
+        }
+    };
+    if (w0 < w1) {
+        const Job a = k.open(w0, b1, r0);
+        if (w0 == b0 && a.pos > 0) join(w0);  // goes on from the block before
+        else if (w0 == b0 && lane == 0) pl.seams[blockIdx.x] = make_int4(-1, 0, 0, 0);
+        const Job z = k.open(w1 - 1, b1, a.r);  // the last job of this share: if it starts here and goes on in the next one
+        const long long start = w1 - 1 - z.pos;
+        if (start >= w0 && start + z.steps > w1) join(start);
+    }
+}
+
+// Jobs that several blocks share.  One block per seam between two blocks of the kernel above.
+template <typename T, int DP>
+__global__ void __launch_bounds__(128) cached_join_kernel(const __grid_constant__ SbCacheParams p, const __grid_constant__ Plan pl) {
+    using K = Kernel<T, DP>;
+    constexpr int N = DP / 32;
+    pdl_wait();
+    pdl_launch_dependents();
+    const int b = blockIdx.x + 1, lane = threadIdx.x & 31;
+    const int4 seam = pl.seams[b];
+    if (seam.x < 0) return;
+    const K k{p, pl, nullptr, lane, p.attend_current ? 1 : 0};
+    Job j;
+    j.r = seam.x;
+    j.g = seam.y;
+    j.tile = seam.z;
+    k.request(j.r, j.first, j.n, j.len);
+    j.cols = min(kCols, j.n * pl.shared - j.tile * kCols);
+    for (int c = threadIdx.x >> 5; c < j.cols; c += 4) {
+        float x[N] = {}, sum = 0.f;
+        for (int a = b - 1; a <= seam.w; ++a) {
+            const float* slot = pl.block_slots + ((size_t)a * 2 + (a < b ? 1 : 0)) * kSlot(DP);
+            const float weight = expf(-sum);
+#pragma unroll
+            for (int i = 0; i < N; ++i) x[i] = fmaf(weight, slot[c * DP + lane * N + i], x[i]);
+            sum += slot[kCols * DP + c];
+        }
+        k.store(j, c, lane * N, x, sum, lane == 0);
+    }
+}
+
+int64_t grid_of(const SbCacheParams& p) {
+    const int64_t all = (int64_t)sm_count() * (p.row == 128 ? 1 : 2);
+    const int64_t shared = p.heads / p.kv_heads, tiles = ((int64_t)p.tokens * shared + kCols - 1) / kCols + p.requests;
+    const int64_t steps = ((int64_t)p.width * p.page_tokens + 31) / 32, most = tiles * (steps > 0 ? steps : 1) * p.kv_heads;  // no more units than this
+    const int64_t want = (most + kWarps - 1) / kWarps;
+    return want < all ? (want < 1 ? 1 : want) : all;
+}
+
+Plan plan_of(const SbCacheParams& p, int64_t grid) {
+    Plan pl;
+    pl.shared = p.heads / p.kv_heads;
+    char* w = (char*)p.workspace;
+    pl.seams = (int4*)w;
+    pl.block_slots = (float*)(w + align_up(16 * (size_t)grid, 256));
+    pl.warp_slots = pl.block_slots + (size_t)grid * 2 * kSlot(p.row);
+    return pl;
+}
+
+template <typename T, int DP>
+int launch(const SbCacheParams& p, cudaStream_t st) {
+    const int64_t grid = grid_of(p);
+    const Plan pl = plan_of(p, grid);
+    CUtensorMap km, vm;
+    const int box = p.page_tokens < 32 ? p.page_tokens : 32;
+    if (encode_page_map(&km, p.k_codes, DP, (int64_t)p.kv_heads * p.page_tokens, p.pages, p.k_stride, box) != 0 ||
+        encode_page_map(&vm, p.v_codes, DP, (int64_t)p.kv_heads * p.page_tokens, p.pages, p.v_stride, box) != 0)
+        return kMapEncodeFailed;
+    int rc = ensure_kernel_attrs((const void*)cached_kernel<T, DP>, (int)Layout<DP>::bytes(SBATTN_MAX_REQUESTS), true);
+    if (rc != 0) return rc;
+    rc = launch_kernel(cached_kernel<T, DP>, dim3((unsigned)grid), dim3(kThreads), Layout<DP>::bytes(p.requests), st, p, pl, km, vm);
+    if (rc != 0 || grid < 2) return rc;
+    return launch_kernel(cached_join_kernel<T, DP>, dim3((unsigned)grid - 1), dim3(128), 0, st, p, pl);
 }
 
 template <typename T>
-int launch(const SbCacheParams& p, cudaStream_t st) {
-    const dim3 grid((unsigned)((p.tokens + kWarps - 1) / kWarps), (unsigned)p.heads);
-    return launch_kernel(cached_kernel<T>, grid, dim3(32 * kWarps), 0, st, p);
+int launch_row(const SbCacheParams& p, cudaStream_t st) {
+    return p.row == 128 ? launch<T, 128>(p, st) : p.row == 64 ? launch<T, 64>(p, st) : launch<T, 32>(p, st);
 }
 
 }  // namespace
 
-size_t cached_workspace(const SbCacheParams&) { return 0; }
+size_t cached_workspace(const SbCacheParams& p) {
+    if (p.heads == 0 || p.kv_heads == 0) return 0;
+    const size_t grid = (size_t)grid_of(p);
+    return align_up(16 * grid, 256) + grid * (2 + 2 * kWarps) * kSlot(p.row) * sizeof(float);
+}
 
 int launch_cached_fwd(const SbCacheParams& p, cudaStream_t st) {
-    if (p.dtype == SBATTN_F32) return launch<float>(p, st);
-    if (p.dtype == SBATTN_F16) return launch<__half>(p, st);
-    return launch<__nv_bfloat16>(p, st);
+    if (p.dtype == SBATTN_F32) return launch_row<float>(p, st);
+    if (p.dtype == SBATTN_F16) return launch_row<__half>(p, st);
+    return launch_row<__nv_bfloat16>(p, st);
 }
 
 }  // namespace sb

@@ -138,6 +138,14 @@ __device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* m, uin
         : "memory");
 }
 
+// 3-d tile load (pages of the 8-bit cache): coordinates (c0 = byte of a row, c1 = row of a page, c2 = page)
+__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* m, uint64_t* bar, int c0, int c1, int c2) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+        ::"r"(smem_u32(dst)), "l"((uint64_t)m), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2)
+        : "memory");
+}
+
 // ---------------------------------------------------------------------------------------------- TMEM
 // one full warp; writes the base address (lane 0, first column) to *dst (shared memory)
 __device__ __forceinline__ void tmem_alloc(uint32_t* dst, uint32_t ncols) {
@@ -321,5 +329,8 @@ __device__ __forceinline__ bool elect_one() {
 // 128-byte swizzle).  Returns 0 on success.
 int encode_tile_map(CUtensorMap* map, const void* ptr, int elem_kind /*0 bf16, 2 f16*/, int64_t D, int64_t T, int64_t H,
                     int64_t B, int64_t stride_t, int64_t stride_h, int64_t stride_b, int box_rows);
+// Pages of the 8-bit cache as [pages][rows][row bytes], page_stride bytes from page to page; a box is box_rows whole rows, swizzled as wide as
+// a row is (rows of 32 bytes are not).
+int encode_page_map(CUtensorMap* map, const void* ptr, int row, int64_t rows, int64_t pages, int64_t page_stride, int box_rows);
 
 }  // namespace sb
