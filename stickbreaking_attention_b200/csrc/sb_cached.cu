@@ -1,8 +1,8 @@
 // Stick-breaking attention of new tokens over the 8-bit paged cache.
 //
-// With s_ij = q_i . k_j * inv_temp, beta = 1 / (1 + exp(-s)) and soft(s) = log(1 + exp(s)) = -log(1 - beta), a query's weights are
-// A_ij = beta_ij exp(-sum of soft over the keys to the right of j that it sees), and two ranges of keys, each treated as if nothing were to its
-// right, join by o = o_right + exp(-S_right) o_left, S = S_right + S_left: no maximum and no renormalisation.  So the keys of all
+// With x_ij = q_i . k_j * inv_temp * log2(e), beta = 1 / (1 + 2^-x) and soft(x) = log2(1 + 2^x) = -log2(1 - beta), a query's weights are
+// A_ij = beta_ij 2^-(sum of soft over the keys to the right of j that it sees), and two ranges of keys, each treated as if nothing were to its
+// right, join by o = o_right + 2^-S_right o_left, S = S_right + S_left: no maximum and no renormalisation.  So the keys of all
 // requests and heads are one line of work, cut into equal shares for all warps of the GPU wherever the cuts fall.
 //
 // What bounds it is the cache's bytes (2 row bytes per key and head, once), as long as few queries share a key.  A warp goes through its share 32
@@ -19,33 +19,41 @@
 #include "sb_cache.cuh"
 #include "sb_sm100.cuh"
 
+#include <cstddef>
+#include <type_traits>
+
 namespace sb {
 
 namespace {
 
 using namespace sm100;
 
-constexpr int kWarps = 8, kThreads = 32 * kWarps;
 constexpr int kCols = 8;       // queries that share a key's product
 constexpr int kColStride = 40; // floats from column to column in the exchange buffer: 4-byte stores and 8-byte loads without bank conflicts
 
-__host__ __device__ constexpr int stages(int dp) { return dp == 32 ? 4 : 3; }
+__host__ __device__ constexpr int warps(int dp) { return dp == 128 ? 12 : 8; }
+__host__ __device__ constexpr int blocks_per_sm(int dp) { return dp == 128 ? 1 : 2; }
+__host__ __device__ constexpr int stages(int dp) { return dp == 32 ? 4 : dp == 64 ? 3 : 2; }
 __host__ __device__ constexpr int stage_bytes(int dp) { return 2 * 32 * dp; }
 
-struct WarpScratch {
+template <int ST>
+struct alignas(16) WarpScratch {
     float x[kCols * kColStride];  // scores, then the two terms of the weights
-    float carry[kCols], carry_low[kCols];  // sum of soft to the right of the present keys, and what rounding it has lost
+    float2 carry[kCols];          // sum of soft to the right of the present keys, and what rounding it has lost
     float factor[kCols];          // power of two that the weights were divided by
-    float temp[kCols];            // inv_temp by what the query was multiplied with
-    float scale[4][4];            // per stage: keys' scale of the lower and upper 16 keys, values' scale
-    uint64_t full[4];
+    float temp[kCols];            // inv_temp log2(e) by what the query was multiplied with
+    int limit[kCols];             // keys that the column sees
+    float scale[ST][4];           // per stage: keys' scale of the lower and upper 16 keys, values' scale
+    uint64_t full[ST];
 };
 
 template <int DP>
 struct Layout {
-    static constexpr size_t ring = (size_t)kWarps * stages(DP) * stage_bytes(DP);
+    static constexpr size_t ring = (size_t)warps(DP) * stages(DP) * stage_bytes(DP);
     static constexpr size_t scratch = ring;
-    static constexpr size_t starts = scratch + kWarps * sizeof(WarpScratch);
+    static constexpr size_t starts = scratch + warps(DP) * sizeof(WarpScratch<stages(DP)>);
+    static_assert(ring % 1024 == 0 && sizeof(WarpScratch<stages(DP)>) % 16 == 0 && offsetof(WarpScratch<stages(DP)>, scale) % 16 == 0, "16-byte accesses");
+    static_assert(1024 + starts + 4 * (SBATTN_MAX_REQUESTS + 1) + 256 <= 232448, "shared memory of a block");
     static size_t bytes(int requests) { return 1024 + starts + sizeof(int) * ((size_t)requests + 1); }  // 1024: the ring is aligned by hand
 };
 __host__ __device__ constexpr int kSlot(int dp) { return kCols * dp + kCols; }  // floats of a partial result: [column][d], then the sums
@@ -60,7 +68,7 @@ struct Job {
 // What the host knows of a launch besides the parameters
 struct Plan {
     int shared;          // queries' heads per key/value head
-    float* warp_slots;   // [grid * kWarps][2] partial results
+    float* warp_slots;   // [grid][warps][2] partial results
     float* block_slots;  // [grid][2]
     int4* seams;         // [grid]: (request or -1, head, tile, last block) of the job that the block's first unit continues, if it started in the block before
 };
@@ -79,6 +87,23 @@ __device__ __forceinline__ void codes_to_f16(uint32_t w, uint32_t& lo, uint32_t&
     asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}" : "=r"(lo), "=r"(hi) : "r"(w));
 }
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }  // -126 <= e <= 127
+
+__device__ __forceinline__ float ex2(float x) {  // 2^x, 2 units of the last place, subnormal results too
+    float y;
+    asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float rcp(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// log2(1 + e) for 0 <= e <= 1, to 3e-7 of itself however small e is: with s = e / (2 + e) it is 2 / ln 2 artanh(s) = s Q(s^2), Q fitted on
+// [0, 1/9] by least squares of the relative error, reweighted until even (4e-9)
+__device__ __forceinline__ float log2_1p(float e) {
+    const float s = e * rcp(2.f + e), z = s * s;
+    return s * fmaf(fmaf(fmaf(fmaf(0.40652743f, z, 0.40338624f), z, 0.57743740f), z, 0.96179163f), z, 2.88539004f);
+}
 
 // Places of rows in a stage.  Rows of 128 and 64 bytes are swizzled by TMA; which keys the lanes of a phase read is chosen so
 // that eight (16-byte loads) or sixteen of them (8-byte) meet all banks once.
@@ -156,7 +181,7 @@ struct Kernel {
     __device__ __forceinline__ void store(const Job& j, int c, int d0, const float (&x)[N], float sum, bool writes_rem) const {
         int h;
         const int t = row_of(j, c, h);
-        const T left = from_f32<T>(expf(-sum));
+        const T left = from_f32<T>(ex2(-sum));
         T* o = (T*)p.o.ptr + h * p.o.stride_h + t * p.o.stride_t;
         const T* v = p.v.ptr ? (const T*)p.v.ptr + j.g * p.v.stride_h + t * p.v.stride_t : nullptr;
 #pragma unroll
@@ -167,17 +192,17 @@ struct Kernel {
 };
 
 template <typename T, int DP>
-__global__ void __launch_bounds__(kThreads, DP == 128 ? 1 : 2)
+__global__ void __launch_bounds__(32 * warps(DP), blocks_per_sm(DP))
 cached_kernel(const __grid_constant__ SbCacheParams p, const __grid_constant__ Plan pl, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
     using K = Kernel<T, DP>;
-    constexpr int ST = K::ST, KW = K::KW, VW = K::VW, M = K::M;
+    constexpr int ST = K::ST, KW = K::KW, VW = K::VW, M = K::M, kWarps = warps(DP), kThreads = 32 * kWarps;
     extern __shared__ uint8_t raw[];
     uint8_t* const sm = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);
     __shared__ long long warp_sums[kWarps];
     __shared__ uint32_t gave_up;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rr = lane >> 2, cc = lane & 3;
     uint8_t* const ring = sm + (size_t)warp * ST * stage_bytes(DP);
-    WarpScratch& ws = ((WarpScratch*)(sm + Layout<DP>::scratch))[warp];
+    WarpScratch<ST>& ws = ((WarpScratch<ST>*)(sm + Layout<DP>::scratch))[warp];
     int* const starts = (int*)(sm + Layout<DP>::starts);
     const int see = p.attend_current ? 1 : 0, P = p.page_tokens, R = p.requests;
     if (lane == 0)
@@ -320,7 +345,7 @@ cached_kernel(const __grid_constant__ SbCacheParams p, const __grid_constant__ P
     int stage = 0;
     uint32_t parity = 0;
     bool alive = true;
-    const int pk = key_of_row<DP>(rr);
+    const int pk = key_of_row<DP>(rr), place = place_of<DP>(lane);
     Job j;
     j.r = r0;
     for (long long u = w0; u < w1 && alive;) {
@@ -328,6 +353,7 @@ cached_kernel(const __grid_constant__ SbCacheParams p, const __grid_constant__ P
         const bool starts_here = j.pos == 0, ends_here = j.end == j.steps;
         u += j.end - j.pos;
         const int least = k.sees(j, 0);  // keys that every column sees
+        const bool packed = j.cols <= kCols / 2;  // the weights' low terms in the other columns
 
         // the queries: column rr, the d's of this lane's words, scaled to at most 2^15
         uint32_t qh[2 * KW], ql[K::kSplitQ ? 2 * KW : 1];
@@ -363,8 +389,9 @@ cached_kernel(const __grid_constant__ SbCacheParams p, const __grid_constant__ P
             }
             __syncwarp();
             if (cc == 0) {
-                ws.temp[rr] = p.inv_temp * pow2(e - 14);
-                ws.carry[rr] = ws.carry_low[rr] = 0.f;
+                ws.temp[rr] = p.inv_temp * 1.44269504f * pow2(e - 14);
+                ws.carry[rr] = make_float2(0.f, 0.f);
+                ws.limit[rr] = k.sees(j, rr);
             }
             __syncwarp();
         }
@@ -385,7 +412,7 @@ cached_kernel(const __grid_constant__ SbCacheParams p, const __grid_constant__ P
             for (int mt = 0; mt < 2; ++mt) {
                 float s[4] = {0.f, 0.f, 0.f, 0.f};
                 const int ka = 16 * mt + pk, kb = ka + 8;
-                uint32_t wa[KW], wb[KW];
+                alignas(16) uint32_t wa[KW], wb[KW];
                 if constexpr (DP == 32) {
                     *(uint2*)wa = *(const uint2*)(kt + ka * 32 + cc * 8);
                     *(uint2*)wb = *(const uint2*)(kt + kb * 32 + cc * 8);
@@ -404,56 +431,71 @@ cached_kernel(const __grid_constant__ SbCacheParams p, const __grid_constant__ P
                     mma16816(s, a0, a1, a2, a3, qh[2 * w], qh[2 * w + 1]);
                     if (K::kSplitQ) mma16816(s, a0, a1, a2, a3, ql[2 * w], ql[2 * w + 1]);
                 }
-                float* const x0 = ws.x + 2 * cc * kColStride + ka;
-                x0[0] = s[0];
-                x0[kColStride] = s[1];
-                x0[8] = s[2];
-                x0[kColStride + 8] = s[3];
+                if (2 * cc < j.cols) {
+                    float* const x0 = ws.x + 2 * cc * kColStride + ka;
+                    x0[0] = s[0];
+                    x0[kColStride] = s[1];
+                    x0[8] = s[2];
+                    x0[kColStride + 8] = s[3];
+                }
             }
             __syncwarp();
-            // weights: a lane has a key
+            // weights: a lane has a key; in powers of two throughout
             const float ks = ws.scale[stage][lane >> 4], vs = ws.scale[stage][2 + (lane >> 4)];
-            const int place = place_of<DP>(lane);
-            for (int c = 0; c < j.cols; ++c) {
-                float* const col = ws.x + c * kColStride;
-                const bool seen = key0 + lane < k.sees(j, c);
-                const float x = col[lane] * (ws.temp[c] * ks);
-                const float e = expf(-fabsf(x));
-                float soft = fmaxf(x, 0.f) + log1pf(e);
-                if (x != x) soft = x;
-                float weight = __fdividef(x >= 0.f ? 1.f : e, 1.f + e);
-                if (!seen) soft = 0.f;
-                float sum = soft;
+            const auto weights = [&](auto count, int c0) {
+                constexpr int C = decltype(count)::value;
+                float weight[C], sum[C];
 #pragma unroll
-                for (int off = 1; off < 32; off <<= 1) {
-                    const float y = __shfl_down_sync(0xffffffffu, sum, off);
-                    if (lane + off < 32) sum += y;
+                for (int i = 0; i < C; ++i) {
+                    const bool seen = key0 + lane < ws.limit[c0 + i];
+                    const float x = ws.x[(c0 + i) * kColStride + lane] * (ws.temp[c0 + i] * ks);
+                    const float e = ex2(-fabsf(x));
+                    sum[i] = seen ? fmaxf(x, 0.f) + log2_1p(e) : 0.f;
+                    weight[i] = seen ? (x >= 0.f ? 1.f : e) * rcp(1.f + e) * vs : 0.f;
                 }
-                float right = __shfl_down_sync(0xffffffffu, sum, 1);
-                if (lane == 31) right = 0.f;
-                const float total = __shfl_sync(0xffffffffu, sum, 0), had = ws.carry[c], low = ws.carry_low[c];
-                weight = seen ? weight * vs * expf(-(had + (low + right))) : 0.f;
-                // to at most 2^15, and in two terms
-                const int e2 = max((int)(__reduce_max_sync(0xffffffffu, __float_as_uint(weight) & 0x7fffffffu) >> 23), 15);
-                const float y = weight * pow2(14 + 127 - e2);
-                const __half hi = __float2half_rn(y);
-                const float rest = y - __half2float(hi);
-                const __half lo = __float2half_rn(fabsf(y) <= 65504.f ? rest : 0.f);
+#pragma unroll
+                for (int off = 1; off < 32; off <<= 1)
+#pragma unroll
+                    for (int i = 0; i < C; ++i) {
+                        const float y = __shfl_down_sync(0xffffffffu, sum[i], off);
+                        if (lane + off < 32) sum[i] += y;
+                    }
+                float right[C], total[C];
+                float2 had[C];
+                int e2[C];
+#pragma unroll
+                for (int i = 0; i < C; ++i) {
+                    right[i] = __shfl_down_sync(0xffffffffu, sum[i], 1);
+                    if (lane == 31) right[i] = 0.f;
+                    total[i] = __shfl_sync(0xffffffffu, sum[i], 0);
+                    had[i] = ws.carry[c0 + i];
+                    right[i] = had[i].x + (had[i].y + right[i]);
+                    weight[i] = weight[i] != 0.f ? weight[i] * ex2(-right[i]) : 0.f;
+                    e2[i] = max((int)(__reduce_max_sync(0xffffffffu, __float_as_uint(weight[i]) & 0x7fffffffu) >> 23), 15);
+                }
                 __syncwarp();
-                ((__half*)col)[place] = hi;
-                ((__half*)col)[32 + place] = lo;
-                if (lane == 0) {
-                    ws.factor[c] = pow2(e2 - 127 - 14);
-                    const float now = had + total, part = now - had;  // two-sum
-                    ws.carry_low[c] = now <= 3.4028234664e38f ? low + ((had - (now - part)) + (total - part)) : 0.f;
-                    ws.carry[c] = now;
+#pragma unroll
+                for (int i = 0; i < C; ++i) {  // to at most 2^15, and in two terms
+                    const float y = weight[i] * pow2(14 + 127 - e2[i]);
+                    const __half hi = __float2half_rn(y), lo = __float2half_rn(fabsf(y) <= 65504.f ? y - __half2float(hi) : 0.f);
+                    __half* const to = (__half*)(ws.x + (c0 + i) * kColStride) + place;
+                    to[0] = hi;
+                    to[packed ? kCols / 2 * kColStride * 2 : 32] = lo;
+                    if (lane == 0) {
+                        ws.factor[c0 + i] = pow2(e2[i] - 127 - 14);
+                        const float now = had[i].x + total[i], part = now - had[i].x;  // two-sum
+                        ws.carry[c0 + i] = make_float2(now, now <= 3.4028234664e38f ? had[i].y + ((had[i].x - (now - part)) + (total[i] - part)) : 0.f);
+                    }
                 }
-            }
+            };
+            int c0 = 0;
+            for (; c0 + 4 <= j.cols; c0 += 4) weights(std::integral_constant<int, 4>(), c0);
+            for (; c0 < j.cols; ++c0) weights(std::integral_constant<int, 1>(), c0);
             __syncwarp();
             // weights times values
             const bool edge = key0 + 32 > least;
             bool mixed_nan = false;
-            uint32_t vw[2][4][VW];
+            alignas(16) uint32_t vw[2][4][VW];
 #pragma unroll
             for (int ks16 = 0; ks16 < 2; ++ks16)
 #pragma unroll
@@ -463,23 +505,32 @@ cached_kernel(const __grid_constant__ SbCacheParams p, const __grid_constant__ P
                     if constexpr (DP == 128) *(uint4*)w = *(const uint4*)(vt + chunk_at<DP>(key, rr));
                     else if constexpr (DP == 64) *(uint2*)w = *(const uint2*)(vt + chunk_at<DP>(key, rr >> 1) + 8 * (rr & 1));
                     else w[0] = *(const uint32_t*)(vt + key * 32 + rr * 4);
-                    if (edge && key0 + key >= least) {  // keys that some columns do not see: 0 * NaN would be NaN
+                }
+            if (edge)  // keys that some columns do not see: 0 * NaN would be NaN
 #pragma unroll
-                        for (int x = 0; x < VW; ++x) {
-                            if (key0 + key >= j.keys) w[x] = 0;
-                            const uint32_t nan = (((w[x] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7;
-                            if (nan) mixed_nan = true;
-                            w[x] &= ~(nan * 255u);
-                        }
+                for (int i = 0; i < 8; ++i) {
+                    const int key = key0 + 16 * (i >> 2) + key_of<DP>(cc, i & 3);
+                    if (key < least) continue;
+#pragma unroll
+                    for (int x = 0; x < VW; ++x) {
+                        uint32_t& w = vw[i >> 2][i & 3][x];
+                        if (key >= j.keys) w = 0;
+                        const uint32_t nan = (((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7;
+                        if (nan) mixed_nan = true;
+                        w &= ~(nan * 255u);
                     }
                 }
-            const float f0 = ws.factor[2 * cc], f1 = ws.factor[2 * cc + 1];
+            const int fc = packed ? 2 * (cc & 1) : 2 * cc;
+            const float f0 = ws.factor[fc], f1 = ws.factor[fc + 1];
             uint32_t bh[2][2], bl[2][2];
 #pragma unroll
             for (int ks16 = 0; ks16 < 2; ++ks16) {
                 const uint2 h = *(const uint2*)((const __half*)(ws.x + rr * kColStride) + 16 * ks16 + 4 * cc);
-                const uint2 l = *(const uint2*)((const __half*)(ws.x + rr * kColStride) + 32 + 16 * ks16 + 4 * cc);
-                bh[ks16][0] = h.x, bh[ks16][1] = h.y, bl[ks16][0] = l.x, bl[ks16][1] = l.y;
+                bh[ks16][0] = h.x, bh[ks16][1] = h.y;
+                if (!packed) {
+                    const uint2 l = *(const uint2*)((const __half*)(ws.x + rr * kColStride) + 32 + 16 * ks16 + 4 * cc);
+                    bl[ks16][0] = l.x, bl[ks16][1] = l.y;
+                }
             }
 #pragma unroll
             for (int w = 0; w < VW; ++w) {
@@ -492,7 +543,7 @@ cached_kernel(const __grid_constant__ SbCacheParams p, const __grid_constant__ P
                         codes_to_f16(__byte_perm(vw[ks16][0][w], vw[ks16][1][w], half ? 0x7362 : 0x5140), a0, a1);
                         codes_to_f16(__byte_perm(vw[ks16][2][w], vw[ks16][3][w], half ? 0x7362 : 0x5140), a2, a3);
                         mma16816(t[half], a0, a1, a2, a3, bh[ks16][0], bh[ks16][1]);
-                        mma16816(t[half], a0, a1, a2, a3, bl[ks16][0], bl[ks16][1]);
+                        if (!packed) mma16816(t[half], a0, a1, a2, a3, bl[ks16][0], bl[ks16][1]);
                     }
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
@@ -513,7 +564,7 @@ cached_kernel(const __grid_constant__ SbCacheParams p, const __grid_constant__ P
                             if ((vt[at] & 127) == 127)
 #pragma unroll
                                 for (int c = 0; c < 2; ++c)
-                                    if (key0 + key < k.sees(j, 2 * cc + c)) acc[m][2 * i + c] = __int_as_float(0x7fc00000);
+                                    if (key0 + key < ws.limit[fc + c]) acc[m][2 * i + c] = __int_as_float(0x7fc00000);
                         }
             }
             __syncwarp();
@@ -524,6 +575,11 @@ cached_kernel(const __grid_constant__ SbCacheParams p, const __grid_constant__ P
             }
         }
         if (!alive) break;
+        if (packed)
+#pragma unroll
+            for (int m = 0; m < M; ++m)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[m][i] += __shfl_xor_sync(0xffffffffu, acc[m][i], 2);
         // the share's part of this job: the result, or a partial one
         float* const slot = pl.warp_slots + ((size_t)(blockIdx.x * kWarps + warp) * 2 + (starts_here ? 1 : 0)) * kSlot(DP);
 #pragma unroll
@@ -536,7 +592,7 @@ cached_kernel(const __grid_constant__ SbCacheParams p, const __grid_constant__ P
                 x[2 * m] = acc[m][c];
                 x[2 * m + 1] = acc[m][2 + c];
             }
-            const float sum = ws.carry[col] + ws.carry_low[col];
+            const float sum = ws.carry[col].x + ws.carry[col].y;
             if (starts_here && ends_here) {
                 k.store(j, col, d0, x, sum, rr == 0);
             } else {
@@ -577,7 +633,7 @@ cached_kernel(const __grid_constant__ SbCacheParams p, const __grid_constant__ P
                 if (s0 >= last) break;
                 if (s0 == s1) continue;
                 const float* slot = pl.warp_slots + ((size_t)(blockIdx.x * kWarps + w) * 2 + (first >= s0 ? 1 : 0)) * kSlot(DP);
-                const float weight = expf(-sum);
+                const float weight = ex2(-sum);
 #pragma unroll
                 for (int i = 0; i < N; ++i) x[i] = fmaf(weight, slot[c * DP + lane * N + i], x[i]);
                 sum += slot[kCols * DP + c];
@@ -628,7 +684,7 @@ __global__ void __launch_bounds__(128) cached_join_kernel(const __grid_constant_
         float x[N] = {}, sum = 0.f;
         for (int a = b - 1; a <= seam.w; ++a) {
             const float* slot = pl.block_slots + ((size_t)a * 2 + (a < b ? 1 : 0)) * kSlot(DP);
-            const float weight = expf(-sum);
+            const float weight = ex2(-sum);
 #pragma unroll
             for (int i = 0; i < N; ++i) x[i] = fmaf(weight, slot[c * DP + lane * N + i], x[i]);
             sum += slot[kCols * DP + c];
@@ -638,7 +694,7 @@ __global__ void __launch_bounds__(128) cached_join_kernel(const __grid_constant_
 }
 
 int64_t grid_of(const SbCacheParams& p) {
-    const int64_t all = (int64_t)sm_count() * (p.row == 128 ? 1 : 2);
+    const int64_t all = (int64_t)sm_count() * blocks_per_sm(p.row), kWarps = warps(p.row);
     const int64_t shared = p.heads / p.kv_heads, tiles = ((int64_t)p.tokens * shared + kCols - 1) / kCols + p.requests;
     const int64_t steps = ((int64_t)p.width * p.page_tokens + 31) / 32, most = tiles * (steps > 0 ? steps : 1) * p.kv_heads;  // no more units than this
     const int64_t want = (most + kWarps - 1) / kWarps;
@@ -666,7 +722,7 @@ int launch(const SbCacheParams& p, cudaStream_t st) {
         return kMapEncodeFailed;
     int rc = ensure_kernel_attrs((const void*)cached_kernel<T, DP>, (int)Layout<DP>::bytes(SBATTN_MAX_REQUESTS), true);
     if (rc != 0) return rc;
-    rc = launch_kernel(cached_kernel<T, DP>, dim3((unsigned)grid), dim3(kThreads), Layout<DP>::bytes(p.requests), st, p, pl, km, vm);
+    rc = launch_kernel(cached_kernel<T, DP>, dim3((unsigned)grid), dim3(32 * warps(DP)), Layout<DP>::bytes(p.requests), st, p, pl, km, vm);
     if (rc != 0 || grid < 2) return rc;
     return launch_kernel(cached_join_kernel<T, DP>, dim3((unsigned)grid - 1), dim3(128), 0, st, p, pl);
 }
@@ -681,7 +737,7 @@ int launch_row(const SbCacheParams& p, cudaStream_t st) {
 size_t cached_workspace(const SbCacheParams& p) {
     if (p.heads == 0 || p.kv_heads == 0) return 0;
     const size_t grid = (size_t)grid_of(p);
-    return align_up(16 * grid, 256) + grid * (2 + 2 * kWarps) * kSlot(p.row) * sizeof(float);
+    return align_up(16 * grid, 256) + grid * (2 + 2 * warps(p.row)) * kSlot(p.row) * sizeof(float);
 }
 
 int launch_cached_fwd(const SbCacheParams& p, cudaStream_t st) {
