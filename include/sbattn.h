@@ -209,7 +209,7 @@ typedef struct SbBlocksParams {
     void* stream;
 } SbBlocksParams;
 
-#define SBATTN_MAX_REQUESTS 4096
+#define SBATTN_MAX_REQUESTS 2048
 
 int sbattn_cache_blocks(const SbBlocksParams* p);
 /* most pieces that `tokens` new tokens of `requests` requests can make */

@@ -3,7 +3,8 @@
 // With x_ij = q_i . k_j * inv_temp * log2(e), beta = 1 / (1 + 2^-x) and soft(x) = log2(1 + 2^x) = -log2(1 - beta), a query's weights are
 // A_ij = beta_ij 2^-(sum of soft over the keys to the right of j that it sees), and two ranges of keys, each treated as if nothing were to its
 // right, join by o = o_right + 2^-S_right o_left, S = S_right + S_left: no maximum and no renormalisation.  So the keys of all
-// requests and heads are one line of work, cut into equal shares for all warps of the GPU wherever the cuts fall.
+// requests and heads are one line of work, cut into equal shares for all warps of the GPU wherever the cuts fall; a second kernel joins what
+// the cuts have parted.
 //
 // What bounds it is the cache's bytes (2 row bytes per key and head, once), as long as few queries share a key.  A warp goes through its share 32
 // keys at a time, from the right:
@@ -36,6 +37,13 @@ __host__ __device__ constexpr int blocks_per_sm(int dp) { return dp == 128 ? 1 :
 __host__ __device__ constexpr int stages(int dp) { return dp == 32 ? 4 : dp == 64 ? 3 : 2; }
 __host__ __device__ constexpr int stage_bytes(int dp) { return 2 * 32 * dp; }
 
+struct Job {
+    int r, g, tile;      // request, key/value head, tile of columns
+    int first, n, len;   // rows of q of the request, tokens
+    int pos, end, steps; // 32-key steps, counted from the right: [pos, end) of steps
+    int cols, keys;      // columns of the tile, keys that its last column sees
+};
+
 template <int ST>
 struct alignas(16) WarpScratch {
     float x[kCols * kColStride];  // scores, then the two terms of the weights
@@ -45,6 +53,7 @@ struct alignas(16) WarpScratch {
     int limit[kCols];             // keys that the column sees
     float scale[ST][4];           // per stage: keys' scale of the lower and upper 16 keys, values' scale
     uint64_t full[ST];
+    Job job[2];                   // the present one and the next one: here, not in registers
 };
 
 template <int DP>
@@ -58,19 +67,13 @@ struct Layout {
 };
 __host__ __device__ constexpr int kSlot(int dp) { return kCols * dp + kCols; }  // floats of a partial result: [column][d], then the sums
 
-struct Job {
-    int r, g, tile;      // request, key/value head, tile of columns
-    int first, n, len;   // rows of q of the request, tokens
-    int pos, end, steps; // 32-key steps, counted from the right: [pos, end) of steps
-    int cols, keys;      // columns of the tile, keys that its last column sees
-};
-
 // What the host knows of a launch besides the parameters
 struct Plan {
     int shared;          // queries' heads per key/value head
-    float* warp_slots;   // [grid][warps][2] partial results
-    float* block_slots;  // [grid][2]
-    int4* seams;         // [grid]: (request or -1, head, tile, last block) of the job that the block's first unit continues, if it started in the block before
+    int quads, pairs;    // q may be read four values at a time; o written, and v read, two at a time
+    int warps;           // of the grid
+    float* slots;        // [warps][2] partial results: of a job that goes on from the share before, and of one that starts here and goes on
+    int4* seams;         // [warps]: (request or -1, head, tile, last share) of the job that a share's first unit goes on with, if it started in the share before
 };
 
 __device__ __forceinline__ long long units_of(const Plan& pl, int len, int n, int see) {  // per key/value head
@@ -132,6 +135,15 @@ struct Kernel {
     const int* starts;  // units per head before each request
     int lane, see;
 
+    // the last request whose units start at or before u
+    __device__ __forceinline__ int find(long long u) const {
+        int lo = 0, hi = p.requests;
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if ((long long)starts[mid] * p.kv_heads <= u) lo = mid; else hi = mid;
+        }
+        return lo;
+    }
     // the job of unit u, up to unit `stop`; r: a request at or before it
     __device__ __forceinline__ Job open(long long u, long long stop, int r) const {
         Job j;
@@ -176,20 +188,71 @@ struct Kernel {
         head = j.g * pl.shared + col % pl.shared;
         return j.first + col / pl.shared;
     }
-    // results of one column: `n` values from d0 on, the sum of soft; `whole`: this thread writes rem
+    // N results of one column from d0 on, and with `writes_rem` what is left of the stick
     template <int N>
     __device__ __forceinline__ void store(const Job& j, int c, int d0, const float (&x)[N], float sum, bool writes_rem) const {
         int h;
         const int t = row_of(j, c, h);
         const T left = from_f32<T>(ex2(-sum));
-        T* o = (T*)p.o.ptr + h * p.o.stride_h + t * p.o.stride_t;
-        const T* v = p.v.ptr ? (const T*)p.v.ptr + j.g * p.v.stride_h + t * p.v.stride_t : nullptr;
+        T* o = (T*)p.o.ptr + h * p.o.stride_h + t * p.o.stride_t + d0;
+        const T* v = p.v.ptr ? (const T*)p.v.ptr + j.g * p.v.stride_h + t * p.v.stride_t + d0 : nullptr;
+        struct alignas(2 * sizeof(T)) Two {
+            T a, b;
+        };
+        if (N > 1 && pl.pairs) {
+            Two w[N / 2 + 1];
+            if (v)
 #pragma unroll
-        for (int i = 0; i < N; ++i)
-            if (d0 + i < p.head_dim) o[d0 + i] = from_f32<T>(v ? fmaf(to_f32(left), to_f32(v[d0 + i]), x[i]) : x[i]);
+                for (int i = 0; i + 1 < N; i += 2)
+                    if (d0 + i < p.head_dim) w[i / 2] = *(const Two*)(v + i);
+#pragma unroll
+            for (int i = 0; i + 1 < N; i += 2)
+                if (d0 + i < p.head_dim) {
+                    const float l = to_f32(left);
+                    *(Two*)(o + i) = v ? Two{from_f32<T>(fmaf(l, to_f32(w[i / 2].a), x[i])), from_f32<T>(fmaf(l, to_f32(w[i / 2].b), x[i + 1]))}
+                                       : Two{from_f32<T>(x[i]), from_f32<T>(x[i + 1])};
+                }
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                if (d0 + i < p.head_dim) o[i] = from_f32<T>(v ? fmaf(to_f32(left), to_f32(v[i]), x[i]) : x[i]);
+        }
         if (writes_rem) ((T*)p.rem.ptr)[h * p.rem.stride_h + t * p.rem.stride_t] = left;
     }
 };
+
+// One column of `count` partial results, from the right, joined by one warp: lane l has the values lane * N ... of x.  slot(a): the a-th one.
+// The loads do not wait for one another.
+template <int DP, int N, typename F>
+__device__ __forceinline__ void join_parts(int count, int c, int lane, F slot, float (&x)[N], float& sum) {
+    sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = 0.f;
+    for (int base = 0; base < count; base += 32) {
+        float s = base + lane < count ? slot(base + lane)[kCols * DP + c] : 0.f;
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) {
+            const float y = __shfl_up_sync(0xffffffffu, s, off);
+            if (lane >= off) s += y;
+        }
+        float right = __shfl_up_sync(0xffffffffu, s, 1);
+        if (lane == 0) right = 0.f;
+        const float weight = ex2(-(sum + right));
+        const int n = min(32, count - base);
+#pragma unroll 8
+        for (int a = 0; a < n; ++a) {
+            const float w = __shfl_sync(0xffffffffu, weight, a);
+            const float* from = slot(base + a) + c * DP + lane * N;
+            alignas(16) float y[N];
+            if constexpr (N == 4) *(float4*)y = *(const float4*)from;
+            else if constexpr (N == 2) *(float2*)y = *(const float2*)from;
+            else y[0] = from[0];
+#pragma unroll
+            for (int i = 0; i < N; ++i) x[i] = fmaf(w, y[i], x[i]);
+        }
+        sum += __shfl_sync(0xffffffffu, s, 31);
+    }
+}
 
 template <typename T, int DP>
 __global__ void __launch_bounds__(32 * warps(DP), blocks_per_sm(DP))
@@ -209,6 +272,10 @@ cached_kernel(const __grid_constant__ SbCacheParams p, const __grid_constant__ P
         for (int s = 0; s < ST; ++s) mbar_init(&ws.full[s], 1);
     if (threadIdx.x == 0) gave_up = 0;
     fence_barrier_init();
+    if (threadIdx.x == 0) {
+        tma_prefetch_desc(&kmap);
+        tma_prefetch_desc(&vmap);
+    }
     pdl_wait();
     pdl_launch_dependents();
 
@@ -249,82 +316,69 @@ cached_kernel(const __grid_constant__ SbCacheParams p, const __grid_constant__ P
     if (carry > 0x7fffffffll) bad = true, carry = 0;
     if (bad) atomicOr(p.status, SBATTN_ST_BAD_SEQLENS);
     __syncthreads();
-    // rem of the rows that belong to no request
-    if (p.ends) {
-        const int first = R > 0 ? max(0, p.ends[R - 1]) : 0;
-        const long long rows = (long long)max(0, p.tokens - first) * p.heads;
-        for (long long i = (long long)blockIdx.x * kThreads + threadIdx.x; i < rows; i += (long long)gridDim.x * kThreads)
-            ((T*)p.rem.ptr)[(i % p.heads) * p.rem.stride_h + (first + i / p.heads) * p.rem.stride_t] = from_f32<T>(0.f);
-    } else {
-        for (long long i = (long long)blockIdx.x * kThreads + threadIdx.x; i < (long long)p.tokens * p.heads; i += (long long)gridDim.x * kThreads) {
-            const int t = (int)(i / p.heads);
-            if (t >= R || p.lengths[t] <= 0) ((T*)p.rem.ptr)[(i % p.heads) * p.rem.stride_h + t * p.rem.stride_t] = from_f32<T>(0.f);
-        }
-    }
-
     const long long units = carry * p.kv_heads;
-    // blocks with work, each with a unit per warp at least where there are so many
-    const long long active = max(1ll, min((long long)gridDim.x, units / kWarps));
-    const long long b0 = min(units, units * blockIdx.x / active), b1 = min(units, units * (blockIdx.x + 1) / active);
-    const long long w0 = b0 + (b1 - b0) * warp / kWarps, w1 = b0 + (b1 - b0) * (warp + 1) / kWarps;
+    // one share of the units per warp, neighbouring ones on different SMs; no warp waits for another from here on
+    const long long shares = max(1ll, min((long long)gridDim.x * kWarps, units)), self = (long long)warp * gridDim.x + blockIdx.x;
+    const long long w1 = min(units, units * (self + 1) / shares);
     const K k{p, pl, starts, lane, see};
-    int r0 = 0;  // the last request whose units start at or before w0
-    {
-        int hi = R;
-        while (hi - r0 > 1) {
-            const int mid = (r0 + hi) >> 1;
-            if ((long long)starts[mid] * p.kv_heads <= w0) r0 = mid; else hi = mid;
-        }
-    }
+    if (lane == 0) pl.seams[self] = make_int4(-1, 0, 0, 0);
 
-    // ---- loads: unit iu is the next one; lane l holds the pages and scales of the l-th step of a batch of 32
-    long long iu = w0;
-    Job ij;
-    ij.r = r0;
-    int istage = 0, ipos = 0, ibatch = 0, iend = 0;
+    // ---- loads: the next step to load is ipos of a job (of request ir, head ig); lane l holds the pages and scales of the l-th step of a batch of 32
+    long long iu = min(units, units * self / shares);
+    int ir = k.find(iu), ig = 0, isteps = 0, ikeys = 0, which = 0;
+    bool pending = false;  // that job has not been taken over by the steps below
+    int istage = 0, ipos = 0, ibatch = 0, iend = 0, loaded = 0;
     int page0 = 0, page1 = 0;
     float4 sc = make_float4(0.f, 0.f, 0.f, 0.f);
     const int box = min(32, P);
-    const auto issue = [&]() {
-        while (ipos >= iend) {  // the next job with steps of its own in this warp's share
-            if (iu >= w1) return;
-            ij = k.open(iu, w1, ij.r);
-            iu += ij.end - ij.pos;
-            ipos = k.first_pos(ij);
-            iend = ij.end;
-            ibatch = ipos;
+    const auto next_job = [&]() {
+        const Job j = k.open(iu, w1, ir);
+        if (j.pos > 0 && lane == 0) {  // the first job of this share: the join kernel's block of this seam takes it if it started in the share before
+            const long long first = iu - j.pos, last = first + j.steps, before = units * (self - 1) / shares;
+            if (first >= before) pl.seams[self] = make_int4(j.r, j.g, j.tile, (int)((last * shares - 1) / units));  // the share of unit last - 1
         }
+        iu += j.end - j.pos;
+        ir = j.r;
+        ig = j.g;
+        isteps = j.steps;
+        ikeys = j.keys;
+        ipos = ibatch = k.first_pos(j);
+        iend = j.end;
+        pending = true;
+        if (lane == 0) ws.job[which ^ 1] = j;
+    };
+    const auto load_step = [&]() {
         if (ipos == ibatch) {
-            const int key = 32 * (ij.steps - 1 - (ipos + lane));  // first key of this lane's step
+            const int key = 32 * (isteps - 1 - (ipos + lane));  // first key of this lane's step
             page0 = page1 = 0;
             sc = make_float4(0.f, 0.f, 0.f, 0.f);
             bool wrong = false;
             if (ipos + lane < iend) {
-                const int* table = p.tables + ij.r * p.table_stride;
-                const auto look = [&](int at, float& ks, float& vs) {
+                const int* table = p.tables + ir * p.table_stride;
+                const auto look = [&](int at) {
                     int page = table[at / P];
                     if (page < 0 || page >= p.pages) {
                         wrong = true;
                         page = 0;
                     }
-                    ks = p.k_scale[page * p.k_scale_stride + ij.g];
-                    vs = p.v_scale[page * p.v_scale_stride + ij.g];
                     return page;
                 };
-                if (key < ij.keys) page0 = look(key, sc.x, sc.z);
-                sc.y = sc.x;
-                sc.w = sc.z;
-                page1 = page0;
-                if (P == 16 && key + 16 < ij.keys) page1 = look(key + 16, sc.y, sc.w);
+                if (key < ikeys) {
+                    page0 = look(key);
+                    page1 = P == 16 && key + 16 < ikeys ? look(key + 16) : page0;
+                    sc.x = p.k_scale[page0 * p.k_scale_stride + ig];
+                    sc.y = p.k_scale[page1 * p.k_scale_stride + ig];
+                    sc.z = p.v_scale[page0 * p.v_scale_stride + ig];
+                    sc.w = p.v_scale[page1 * p.v_scale_stride + ig];
+                }
             }
             if (wrong) atomicOr(p.status, SBATTN_ST_BAD_PAGES);
             ibatch += 32;
         }
         if (lane == ((ipos - (ibatch - 32)) & 31)) {
-            const int key = 32 * (ij.steps - 1 - ipos), row = ij.g * P + key % P;
+            const int key = 32 * (isteps - 1 - ipos), row = ig * P + key % P;
             uint8_t* const dst = ring + istage * stage_bytes(DP);
-            const bool load = key < ij.keys, two = P == 16 && key + 16 < ij.keys;
-            *(float4*)ws.scale[istage] = sc;
+            const bool load = key < ikeys, two = P == 16 && key + 16 < ikeys;
             mbar_expect_tx(&ws.full[istage], (load ? 2 * box * DP : 0) + (two ? 2 * box * DP : 0));
             if (load) {
                 tma_load_3d(dst, &kmap, &ws.full[istage], 0, row, page0);
@@ -334,44 +388,75 @@ cached_kernel(const __grid_constant__ SbCacheParams p, const __grid_constant__ P
                 tma_load_3d(dst + 16 * DP, &kmap, &ws.full[istage], 0, row, page1);
                 tma_load_3d(dst + 48 * DP, &vmap, &ws.full[istage], 0, row, page1);
             }
+            *(float4*)ws.scale[istage] = sc;  // read by this warp alone, behind a __syncwarp
         }
         ++ipos;
+        ++loaded;
         if (++istage == ST) istage = 0;
     };
-    if (w0 < w1)
-        for (int s = 0; s < ST; ++s) issue();
 
     // ---- steps
     int stage = 0;
     uint32_t parity = 0;
-    bool alive = true;
+    bool alive = true, working = false;
     const int pk = key_of_row<DP>(rr), place = place_of<DP>(lane);
-    Job j;
-    j.r = r0;
-    for (long long u = w0; u < w1 && alive;) {
-        j = k.open(u, w1, j.r);
-        const bool starts_here = j.pos == 0, ends_here = j.end == j.steps;
-        u += j.end - j.pos;
-        const int least = k.sees(j, 0);  // keys that every column sees
-        const bool packed = j.cols <= kCols / 2;  // the weights' low terms in the other columns
-
-        // the queries: column rr, the d's of this lane's words, scaled to at most 2^15
-        uint32_t qh[2 * KW], ql[K::kSplitQ ? 2 * KW : 1];
-        {
-            float x[4 * KW];
-            float top = 0.f;
+    int pos = 0, end = 0, steps = 0, cols = 0, keys = 0, least = 0;
+    bool packed = false;
+    uint32_t qh[2 * KW], ql[K::kSplitQ ? 2 * KW : 1];
+    float acc[M][4];
+    for (;;) {
+        while (loaded < ST) {
+            if (ipos < iend) load_step();
+            else if (!pending && iu < w1) next_job();
+            else break;
+        }
+        if (!working) {
+            if (!pending) break;
+            // the next job: its queries, scaled to at most 2^15
+            which ^= 1;
+            __syncwarp();
+            const Job cj = ws.job[which];
+            pending = false;
+            working = true;
+            pos = k.first_pos(cj);
+            end = cj.end;
+            steps = cj.steps;
+            cols = cj.cols;
+            keys = cj.keys;
+            least = k.sees(cj, 0);  // keys that every column sees
+            packed = cols <= kCols / 2;  // the weights' low terms in the other columns
+            struct alignas(4 * sizeof(T)) Four {
+                T a, b, c, d;
+            } nq[KW];  // column rr, the d's of this lane's words
             int h = 0, t = 0;
-            if (rr < j.cols) t = k.row_of(j, rr, h);
+            if (rr < cj.cols) t = k.row_of(cj, rr, h);
             const T* q = (const T*)p.q.ptr + h * p.q.stride_h + t * p.q.stride_t;
 #pragma unroll
             for (int w = 0; w < KW; ++w) {
                 const int d = DP == 128 ? 16 * (cc + 4 * (w >> 2)) + 4 * (w & 3) : DP == 64 ? 16 * cc + 4 * w : 8 * cc + 4 * w;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    x[4 * w + i] = rr < j.cols && d + i < p.head_dim ? to_f32(q[d + i]) : 0.f;
-                    const float a = fabsf(x[4 * w + i]);
-                    if (a <= 3.4028234664e38f) top = fmaxf(top, a);
+                nq[w] = Four{T(0.f), T(0.f), T(0.f), T(0.f)};
+                if (rr < cj.cols) {
+                    if (pl.quads) {
+                        if (d < p.head_dim) nq[w] = *(const Four*)(q + d);
+                    } else {
+                        if (d < p.head_dim) nq[w].a = q[d];
+                        if (d + 1 < p.head_dim) nq[w].b = q[d + 1];
+                        if (d + 2 < p.head_dim) nq[w].c = q[d + 2];
+                        if (d + 3 < p.head_dim) nq[w].d = q[d + 3];
+                    }
                 }
+            }
+            float top = 0.f;
+            const auto take = [&](T x) {
+                const float a = fabsf(to_f32(x));
+                if (a <= 3.4028234664e38f) top = fmaxf(top, a);
+            };
+#pragma unroll
+            for (int w = 0; w < KW; ++w) {
+                take(nq[w].a);
+                take(nq[w].b);
+                take(nq[w].c);
+                take(nq[w].d);
             }
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
@@ -379,7 +464,8 @@ cached_kernel(const __grid_constant__ SbCacheParams p, const __grid_constant__ P
             const float up = pow2(14 - e);
 #pragma unroll
             for (int i = 0; i < 2 * KW; ++i) {
-                const float a = x[2 * i] * up, b = x[2 * i + 1] * up;
+                const Four& f = nq[i >> 1];
+                const float a = to_f32(i & 1 ? f.c : f.a) * up, b = to_f32(i & 1 ? f.d : f.b) * up;
                 qh[i] = pack_f16(a, b);
                 if (K::kSplitQ) {
                     const __half2 hi = *(const __half2*)&qh[i];
@@ -391,20 +477,20 @@ cached_kernel(const __grid_constant__ SbCacheParams p, const __grid_constant__ P
             if (cc == 0) {
                 ws.temp[rr] = p.inv_temp * 1.44269504f * pow2(e - 14);
                 ws.carry[rr] = make_float2(0.f, 0.f);
-                ws.limit[rr] = k.sees(j, rr);
+                ws.limit[rr] = rr < cj.cols ? k.sees(cj, rr) : 0;
             }
             __syncwarp();
-        }
-        float acc[M][4];
 #pragma unroll
-        for (int m = 0; m < M; ++m) acc[m][0] = acc[m][1] = acc[m][2] = acc[m][3] = 0.f;
-
-        for (int pos = k.first_pos(j); pos < j.end; ++pos) {
-            const int key0 = 32 * (j.steps - 1 - pos);
+            for (int m = 0; m < M; ++m) acc[m][0] = acc[m][1] = acc[m][2] = acc[m][3] = 0.f;
+            continue;
+        }
+        if (pos < end) {
+            const int key0 = 32 * (steps - 1 - pos);
             if (!mbar_wait(&ws.full[stage], parity, &gave_up)) {
                 alive = false;
                 break;
             }
+            __syncwarp();
             const uint8_t* const kt = ring + stage * stage_bytes(DP);
             const uint8_t* const vt = kt + 32 * DP;
             // scores: 2 x 16 keys by 8 columns
@@ -431,7 +517,7 @@ cached_kernel(const __grid_constant__ SbCacheParams p, const __grid_constant__ P
                     mma16816(s, a0, a1, a2, a3, qh[2 * w], qh[2 * w + 1]);
                     if (K::kSplitQ) mma16816(s, a0, a1, a2, a3, ql[2 * w], ql[2 * w + 1]);
                 }
-                if (2 * cc < j.cols) {
+                if (2 * cc < cols) {
                     float* const x0 = ws.x + 2 * cc * kColStride + ka;
                     x0[0] = s[0];
                     x0[kColStride] = s[1];
@@ -488,9 +574,9 @@ cached_kernel(const __grid_constant__ SbCacheParams p, const __grid_constant__ P
                     }
                 }
             };
-            int c0 = 0;
-            for (; c0 + 4 <= j.cols; c0 += 4) weights(std::integral_constant<int, 4>(), c0);
-            for (; c0 < j.cols; ++c0) weights(std::integral_constant<int, 1>(), c0);
+            if (cols == 1) weights(std::integral_constant<int, 1>(), 0);
+            else
+                for (int c0 = 0; c0 < cols; c0 += 4) weights(std::integral_constant<int, 4>(), c0);  // those behind the last see nothing
             __syncwarp();
             // weights times values
             const bool edge = key0 + 32 > least;
@@ -514,7 +600,7 @@ cached_kernel(const __grid_constant__ SbCacheParams p, const __grid_constant__ P
 #pragma unroll
                     for (int x = 0; x < VW; ++x) {
                         uint32_t& w = vw[i >> 2][i & 3][x];
-                        if (key >= j.keys) w = 0;
+                        if (key >= keys) w = 0;
                         const uint32_t nan = (((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7;
                         if (nan) mixed_nan = true;
                         w &= ~(nan * 255u);
@@ -555,7 +641,7 @@ cached_kernel(const __grid_constant__ SbCacheParams p, const __grid_constant__ P
                 }
             }
             if (edge && __any_sync(0xffffffffu, mixed_nan)) {  // NaN for the columns that do see them
-                for (int key = max(0, least - key0); key < min(32, j.keys - key0); ++key)
+                for (int key = max(0, least - key0); key < min(32, keys - key0); ++key)
 #pragma unroll
                     for (int m = 0; m < M; ++m)
 #pragma unroll
@@ -568,24 +654,28 @@ cached_kernel(const __grid_constant__ SbCacheParams p, const __grid_constant__ P
                         }
             }
             __syncwarp();
-            issue();
+            ++pos;
+            --loaded;
             if (++stage == ST) {
                 stage = 0;
                 parity ^= 1;
             }
+            if (pos < end) continue;
         }
-        if (!alive) break;
+        // the share's part of this job: the result, or a partial one
+        working = false;
+        const Job cj = ws.job[which];
+        const bool starts_here = cj.pos == 0;
         if (packed)
 #pragma unroll
             for (int m = 0; m < M; ++m)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) acc[m][i] += __shfl_xor_sync(0xffffffffu, acc[m][i], 2);
-        // the share's part of this job: the result, or a partial one
-        float* const slot = pl.warp_slots + ((size_t)(blockIdx.x * kWarps + warp) * 2 + (starts_here ? 1 : 0)) * kSlot(DP);
+        float* const slot = pl.slots + ((size_t)self * 2 + (starts_here ? 1 : 0)) * kSlot(DP);
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
             const int col = 2 * cc + c, d0 = rr * 4 * VW;
-            if (col >= j.cols) continue;
+            if (col >= cj.cols) continue;
             float x[2 * M];
 #pragma unroll
             for (int m = 0; m < M; ++m) {
@@ -593,11 +683,11 @@ cached_kernel(const __grid_constant__ SbCacheParams p, const __grid_constant__ P
                 x[2 * m + 1] = acc[m][2 + c];
             }
             const float sum = ws.carry[col].x + ws.carry[col].y;
-            if (starts_here && ends_here) {
-                k.store(j, col, d0, x, sum, rr == 0);
+            if (starts_here && cj.end == cj.steps) {
+                k.store(cj, col, d0, x, sum, rr == 0);
             } else {
 #pragma unroll
-                for (int i = 0; i < 2 * M; ++i) slot[col * DP + d0 + i] = x[i];
+                for (int i = 0; i < M / 2; ++i) *(float4*)(slot + col * DP + d0 + 4 * i) = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
                 if (rr == 0) slot[kCols * DP + col] = sum;
             }
         }
@@ -605,72 +695,42 @@ cached_kernel(const __grid_constant__ SbCacheParams p, const __grid_constant__ P
     }
     if (!alive) {  // no load of this warp may arrive after it has left
         uint32_t ignored = 0;
-        for (int s = 0; s < ST; ++s) {
+        for (; loaded > 0; --loaded) {
             mbar_wait(&ws.full[stage], parity, &ignored);
             if (++stage == ST) {
                 stage = 0;
                 parity ^= 1;
             }
         }
-        if (lane == 0) atomicOr(p.status, SBATTN_ST_TIMEOUT);
+        if (lane == 0) {
+            pl.seams[self] = make_int4(-1, 0, 0, 0);
+            atomicOr(p.status, SBATTN_ST_TIMEOUT);
+        }
     }
 
-    // ---- jobs that several warps of this block share: joined by the warp that has their first part here
-    __syncthreads();
-    if (gave_up || b0 >= b1) {
-        if (threadIdx.x == 0) pl.seams[blockIdx.x] = make_int4(-1, 0, 0, 0);
-        return;
-    }
-    constexpr int N = DP / 32;
-    const auto join = [&](long long u) {  // the job of unit u, the first of its units in this warp's share
-        const Job j = k.open(u, b1, r0);
-        const long long first = u - j.pos, last = first + j.steps;  // the job's units
-        const bool from_before = first < b0, goes_on = last > b1;
-        for (int c = 0; c < j.cols; ++c) {
-            float x[N] = {}, sum = 0.f;
-            for (int w = warp; w < kWarps; ++w) {
-                const long long s0 = b0 + (b1 - b0) * w / kWarps, s1 = b0 + (b1 - b0) * (w + 1) / kWarps;
-                if (s0 >= last) break;
-                if (s0 == s1) continue;
-                const float* slot = pl.warp_slots + ((size_t)(blockIdx.x * kWarps + w) * 2 + (first >= s0 ? 1 : 0)) * kSlot(DP);
-                const float weight = ex2(-sum);
-#pragma unroll
-                for (int i = 0; i < N; ++i) x[i] = fmaf(weight, slot[c * DP + lane * N + i], x[i]);
-                sum += slot[kCols * DP + c];
-            }
-            if (!from_before && !goes_on) {
-                k.store(j, c, lane * N, x, sum, lane == 0);
-            } else {
-                float* slot = pl.block_slots + ((size_t)blockIdx.x * 2 + (from_before ? 0 : 1)) * kSlot(DP);
-#pragma unroll
-                for (int i = 0; i < N; ++i) slot[c * DP + lane * N + i] = x[i];
-                if (lane == 0) slot[kCols * DP + c] = sum;
-            }
-        }
-        if (lane == 0 && from_before) {  // the join kernel's block of this seam takes the job if it started in the block before
-            const long long before = units * ((long long)blockIdx.x - 1) / active;
-            const int last_block = (int)((last * active - 1) / units);  // of unit last - 1
-            pl.seams[blockIdx.x] = first >= before ? make_int4(j.r, j.g, j.tile, last_block) : make_int4(-1, 0, 0, 0);
-        }
-    };
-    if (w0 < w1) {
-        const Job a = k.open(w0, b1, r0);
-        if (w0 == b0 && a.pos > 0) join(w0);  // goes on from the block before
-        else if (w0 == b0 && lane == 0) pl.seams[blockIdx.x] = make_int4(-1, 0, 0, 0);
-        const Job z = k.open(w1 - 1, b1, a.r);  // the last job of this share: if it starts here and goes on in the next one
-        const long long start = w1 - 1 - z.pos;
-        if (start >= w0 && start + z.steps > w1) join(start);
+    // rem of the rows that belong to no request
+    if (p.ends) {
+        const int first = R > 0 ? max(0, p.ends[R - 1]) : 0;
+        const long long rows = (long long)max(0, p.tokens - first) * p.heads;
+        for (long long i = (long long)blockIdx.x * kThreads + threadIdx.x; i < rows; i += (long long)gridDim.x * kThreads)
+            ((T*)p.rem.ptr)[(i % p.heads) * p.rem.stride_h + (first + i / p.heads) * p.rem.stride_t] = from_f32<T>(0.f);
+    } else {
+        for (int t = blockIdx.x * kThreads + threadIdx.x; t < p.tokens; t += gridDim.x * kThreads)
+            if (t >= R || p.lengths[t] <= 0)
+                for (int h = 0; h < p.heads; ++h) ((T*)p.rem.ptr)[h * p.rem.stride_h + t * p.rem.stride_t] = from_f32<T>(0.f);
     }
 }
 
-// Jobs that several blocks share.  One block per seam between two blocks of the kernel above.
+// Jobs that several shares have parts of.  One block per seam between two shares: its warps take the columns, and where there are few of them, parts
+// of the line of partial results, which meet in shared memory.
 template <typename T, int DP>
-__global__ void __launch_bounds__(128) cached_join_kernel(const __grid_constant__ SbCacheParams p, const __grid_constant__ Plan pl) {
+__global__ void __launch_bounds__(32 * kCols) cached_join_kernel(const __grid_constant__ SbCacheParams p, const __grid_constant__ Plan pl) {
     using K = Kernel<T, DP>;
     constexpr int N = DP / 32;
+    __shared__ float xs[kCols][DP], sums[kCols];
     pdl_wait();
     pdl_launch_dependents();
-    const int b = blockIdx.x + 1, lane = threadIdx.x & 31;
+    const int b = blockIdx.x + 1, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int4 seam = pl.seams[b];
     if (seam.x < 0) return;
     const K k{p, pl, nullptr, lane, p.attend_current ? 1 : 0};
@@ -680,34 +740,45 @@ __global__ void __launch_bounds__(128) cached_join_kernel(const __grid_constant_
     j.tile = seam.z;
     k.request(j.r, j.first, j.n, j.len);
     j.cols = min(kCols, j.n * pl.shared - j.tile * kCols);
-    for (int c = threadIdx.x >> 5; c < j.cols; c += 4) {
-        float x[N] = {}, sum = 0.f;
-        for (int a = b - 1; a <= seam.w; ++a) {
-            const float* slot = pl.block_slots + ((size_t)a * 2 + (a < b ? 1 : 0)) * kSlot(DP);
+    const int count = seam.w - b + 2, splits = j.cols <= 1 ? 8 : j.cols <= 2 ? 4 : j.cols <= 4 ? 2 : 1;
+    const int c = warp / splits, part = warp % splits, a0 = count * part / splits, a1 = count * (part + 1) / splits;
+    float x[N], sum = 0.f;
+    if (c < j.cols)
+        join_parts<DP>(a1 - a0, c, lane, [&](int a) { return pl.slots + ((size_t)(b - 1 + a0 + a) * 2 + (a0 + a == 0 ? 1 : 0)) * kSlot(DP); }, x, sum);
+    if (splits > 1) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) xs[warp][lane * N + i] = x[i];
+        if (lane == 0) sums[warp] = sum;
+        __syncthreads();
+        if (part != 0) return;
+        for (int s = 1; s < splits; ++s) {
             const float weight = ex2(-sum);
 #pragma unroll
-            for (int i = 0; i < N; ++i) x[i] = fmaf(weight, slot[c * DP + lane * N + i], x[i]);
-            sum += slot[kCols * DP + c];
+            for (int i = 0; i < N; ++i) x[i] = fmaf(weight, xs[warp + s][lane * N + i], x[i]);
+            sum += sums[warp + s];
         }
-        k.store(j, c, lane * N, x, sum, lane == 0);
     }
+    if (c < j.cols) k.store(j, c, lane * N, x, sum, lane == 0);
 }
 
 int64_t grid_of(const SbCacheParams& p) {
-    const int64_t all = (int64_t)sm_count() * blocks_per_sm(p.row), kWarps = warps(p.row);
+    const int64_t all = (int64_t)sm_count() * blocks_per_sm(p.row);
     const int64_t shared = p.heads / p.kv_heads, tiles = ((int64_t)p.tokens * shared + kCols - 1) / kCols + p.requests;
     const int64_t steps = ((int64_t)p.width * p.page_tokens + 31) / 32, most = tiles * (steps > 0 ? steps : 1) * p.kv_heads;  // no more units than this
-    const int64_t want = (most + kWarps - 1) / kWarps;
-    return want < all ? (want < 1 ? 1 : want) : all;
+    return most < all ? (most < 1 ? 1 : most) : all;
 }
 
 Plan plan_of(const SbCacheParams& p, int64_t grid) {
     Plan pl;
     pl.shared = p.heads / p.kv_heads;
+    const int64_t size = p.dtype == SBATTN_F32 ? 4 : 2;
+    const auto even = [&](const SbMat& m, int n) { return (((uintptr_t)m.ptr | (uintptr_t)(m.stride_h * size) | (uintptr_t)(m.stride_t * size)) & (n * size - 1)) == 0; };
+    pl.quads = p.head_dim % 4 == 0 && even(p.q, 4);
+    pl.pairs = p.head_dim % 2 == 0 && even(p.o, 2) && even(p.v, 2);
+    pl.warps = (int)grid * warps(p.row);
     char* w = (char*)p.workspace;
     pl.seams = (int4*)w;
-    pl.block_slots = (float*)(w + align_up(16 * (size_t)grid, 256));
-    pl.warp_slots = pl.block_slots + (size_t)grid * 2 * kSlot(p.row);
+    pl.slots = (float*)(w + align_up(16 * (size_t)pl.warps, 256));
     return pl;
 }
 
@@ -723,8 +794,8 @@ int launch(const SbCacheParams& p, cudaStream_t st) {
     int rc = ensure_kernel_attrs((const void*)cached_kernel<T, DP>, (int)Layout<DP>::bytes(SBATTN_MAX_REQUESTS), true);
     if (rc != 0) return rc;
     rc = launch_kernel(cached_kernel<T, DP>, dim3((unsigned)grid), dim3(32 * warps(DP)), Layout<DP>::bytes(p.requests), st, p, pl, km, vm);
-    if (rc != 0 || grid < 2) return rc;
-    return launch_kernel(cached_join_kernel<T, DP>, dim3((unsigned)grid - 1), dim3(128), 0, st, p, pl);
+    if (rc != 0) return rc;
+    return launch_kernel(cached_join_kernel<T, DP>, dim3((unsigned)pl.warps - 1), dim3(32 * kCols), 0, st, p, pl);
 }
 
 template <typename T>
@@ -736,8 +807,8 @@ int launch_row(const SbCacheParams& p, cudaStream_t st) {
 
 size_t cached_workspace(const SbCacheParams& p) {
     if (p.heads == 0 || p.kv_heads == 0) return 0;
-    const size_t grid = (size_t)grid_of(p);
-    return align_up(16 * grid, 256) + grid * (2 + 2 * warps(p.row)) * kSlot(p.row) * sizeof(float);
+    const size_t n = (size_t)grid_of(p) * warps(p.row);
+    return align_up(16 * n, 256) + n * 2 * kSlot(p.row) * sizeof(float);
 }
 
 int launch_cached_fwd(const SbCacheParams& p, cudaStream_t st) {

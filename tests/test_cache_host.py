@@ -27,7 +27,7 @@ def blocks_params(**kw):  # its addresses are never followed: every call below i
 
 @pytest.mark.parametrize("change, code", [
     (dict(requests=-1), -1), (dict(width=-1), -1), (dict(pages=-1), -1), (dict(tokens=-1), -1), (dict(page_tokens=24), -1), (dict(page_tokens=0), -1),
-    (dict(table_stride=3), -1), (dict(n_pieces=3), -1), (dict(requests=4097, n_pieces=9000), -3), (dict(width=1 << 27, table_stride=1 << 27), -3),
+    (dict(table_stride=3), -1), (dict(n_pieces=3), -1), (dict(requests=2049, n_pieces=9000), -3), (dict(width=1 << 27, table_stride=1 << 27), -3),
     (dict(tokens=(1 << 30) + 1, n_pieces=1 << 30), -3), (dict(lengths=None), -2), (dict(new_tokens=None), -2), (dict(free_count=None), -2), (dict(tables=None), -2),
     (dict(free_pages=None), -2), (dict(lengths_out=None), -2), (dict(free_count_out=None), -2), (dict(ends=None), -2), (dict(slots=None), -2),
     (dict(pieces=None), -2), (dict(pieces=4100), -5), (dict(status=None), -2)])
@@ -60,7 +60,7 @@ def test_append_refusals(lib, change, code):
 
 
 @pytest.mark.parametrize("change, code", COMMON + [
-    (dict(heads=3), -1), (dict(heads=-2), -1), (dict(kv_heads=0), -1), (dict(requests=-1), -1), (dict(requests=4097), -3), (dict(width=1 << 27, table_stride=1 << 27), -3),
+    (dict(heads=3), -1), (dict(heads=-2), -1), (dict(kv_heads=0), -1), (dict(requests=-1), -1), (dict(requests=2049), -3), (dict(width=1 << 27, table_stride=1 << 27), -3),
     (dict(table_stride=1), -1), (dict(lengths=None), -2), (dict(tables=None), -2), (dict(ends=None, tokens=1), -1)])
 def test_attend_refusals(lib, change, code):
     assert lib.sbattn_cached_fwd(cache_params(**change)) == code
