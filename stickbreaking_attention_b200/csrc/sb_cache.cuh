@@ -34,6 +34,8 @@ __device__ inline float from_e4m3(uint8_t c) { return __half2float(__half(__nv_c
 int launch_cache_blocks(const SbBlocksParams& p, cudaStream_t st);
 int launch_cache_append(const SbCacheParams& p, cudaStream_t st);
 size_t cached_workspace(const SbCacheParams& p);
+size_t cached_tc_workspace(const SbCacheParams& p);
+int launch_cached_tc(const SbCacheParams& p, cudaStream_t st);
 int launch_cached_fwd(const SbCacheParams& p, cudaStream_t st);
 
 }  // namespace sb

@@ -17,7 +17,7 @@
 //   * the weights of 32 keys, with the scale of the values' page, are scaled by a power of two to at most 2^15 per column and split into two float16 terms
 //     (22 bits: what is lost is below float32's own rounding of the sums), the two products are added to float32 accumulators.
 // float32 queries are two float16 terms, too; 16-bit ones are scaled by a power of two per row and exact.
-#include "sb_cache.cuh"
+#include "sb_cached.cuh"
 #include "sb_sm100.cuh"
 
 #include <cstddef>
@@ -28,6 +28,7 @@ namespace sb {
 namespace {
 
 using namespace sm100;
+using namespace cached;
 
 constexpr int kCols = 8;       // queries that share a key's product
 constexpr int kColStride = 40; // floats from column to column in the exchange buffer: 4-byte stores and 8-byte loads without bank conflicts
@@ -36,13 +37,6 @@ __host__ __device__ constexpr int warps(int dp) { return dp == 128 ? 12 : 8; }
 __host__ __device__ constexpr int blocks_per_sm(int dp) { return dp == 128 ? 1 : 2; }
 __host__ __device__ constexpr int stages(int dp) { return dp == 32 ? 4 : dp == 64 ? 3 : 2; }
 __host__ __device__ constexpr int stage_bytes(int dp) { return 2 * 32 * dp; }
-
-struct Job {
-    int r, g, tile;      // request, key/value head, tile of columns
-    int first, n, len;   // rows of q of the request, tokens
-    int pos, end, steps; // 32-key steps, counted from the right: [pos, end) of steps
-    int cols, keys;      // columns of the tile, keys that its last column sees
-};
 
 template <int ST>
 struct alignas(16) WarpScratch {
@@ -65,41 +59,10 @@ struct Layout {
     static_assert(1024 + starts + 4 * (SBATTN_MAX_REQUESTS + 1) + 256 <= 232448, "shared memory of a block");
     static size_t bytes(int requests) { return 1024 + starts + sizeof(int) * ((size_t)requests + 1); }  // 1024: the ring is aligned by hand
 };
-__host__ __device__ constexpr int kSlot(int dp) { return kCols * dp + kCols; }  // floats of a partial result: [column][d], then the sums
-
-// What the host knows of a launch besides the parameters
-struct Plan {
-    int shared;          // queries' heads per key/value head
-    int quads, pairs;    // q may be read four values at a time; o written, and v read, two at a time
-    int warps;           // of the grid
-    float* slots;        // [warps][2] partial results: of a job that goes on from the share before, and of one that starts here and goes on
-    int4* seams;         // [warps]: (request or -1, head, tile, last share) of the job that a share's first unit goes on with, if it started in the share before
-};
-
-__device__ __forceinline__ long long units_of(const Plan& pl, int len, int n, int see) {  // per key/value head
-    const int tiles = (n * pl.shared + kCols - 1) / kCols, keys = len - 1 + see;
-    return (long long)tiles * max(1, (keys + 31) >> 5);
-}
 
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-// four codes to two pairs of float16
-__device__ __forceinline__ void codes_to_f16(uint32_t w, uint32_t& lo, uint32_t& hi) {
-    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}" : "=r"(lo), "=r"(hi) : "r"(w));
-}
-__device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }  // -126 <= e <= 127
-
-__device__ __forceinline__ float ex2(float x) {  // 2^x, 2 units of the last place, subnormal results too
-    float y;
-    asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-__device__ __forceinline__ float rcp(float x) {
-    float y;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
 }
 // log2(1 + e) for 0 <= e <= 1, to 3e-7 of itself however small e is: with s = e / (2 + e) it is 2 / ln 2 artanh(s) = s Q(s^2), Q fitted on
 // [0, 1/9] by least squares of the relative error, reweighted until even (4e-9)
@@ -127,147 +90,19 @@ template <int DP> __device__ __forceinline__ int place_of(int key) {  // 16 * ha
 }
 
 template <typename T, int DP>
-struct Kernel {
-    static constexpr int ST = stages(DP), KW = DP / 16, VW = DP / 32, M = DP / 16;
-    static constexpr bool kSplitQ = sizeof(T) == 4;
-    const SbCacheParams& p;
-    const Plan& pl;
-    const int* starts;  // units per head before each request
-    int lane, see;
-
-    // the last request whose units start at or before u
-    __device__ __forceinline__ int find(long long u) const {
-        int lo = 0, hi = p.requests;
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if ((long long)starts[mid] * p.kv_heads <= u) lo = mid; else hi = mid;
-        }
-        return lo;
-    }
-    // the job of unit u, up to unit `stop`; r: a request at or before it
-    __device__ __forceinline__ Job open(long long u, long long stop, int r) const {
-        Job j;
-        while ((long long)starts[r + 1] * p.kv_heads <= u) ++r;
-        j.r = r;
-        request(r, j.first, j.n, j.len);
-        const int tiles = (j.n * pl.shared + kCols - 1) / kCols;
-        j.steps = max(1, (j.len - 1 + see + 31) >> 5);
-        const unsigned long long in = (unsigned long long)(u - (long long)starts[r] * p.kv_heads);
-        unsigned long long job;
-        if (in >> 32) {
-            job = in / (unsigned)j.steps;
-            j.pos = (int)(in % (unsigned)j.steps);
-        } else {
-            job = (unsigned)in / (unsigned)j.steps;
-            j.pos = (int)((unsigned)in % (unsigned)j.steps);
-        }
-        j.g = (int)(job / (unsigned)tiles);
-        j.tile = (int)(job % (unsigned)tiles);
-        j.end = (int)min((long long)j.steps, j.pos + (stop - u));
-        j.cols = min(kCols, j.n * pl.shared - j.tile * kCols);
-        j.keys = j.len - j.n + (j.tile * kCols + j.cols - 1) / pl.shared + see;
-        return j;
-    }
-    __device__ __forceinline__ void request(int r, int& first, int& n, int& len) const {
-        len = p.lengths[r];
-        if (p.ends) {
-            first = r > 0 ? p.ends[r - 1] : 0;
-            n = p.ends[r] - first;
-        } else {
-            first = r;
-            n = len > 0 ? 1 : 0;
-        }
-    }
-    // first step, counted from the right, that holds a key which the tile sees
-    __device__ __forceinline__ int first_pos(const Job& j) const { return max(j.pos, j.steps - max(1, (j.keys + 31) >> 5)); }
-    // keys that column c of the tile sees
-    __device__ __forceinline__ int sees(const Job& j, int c) const { return j.len - j.n + (j.tile * kCols + c) / pl.shared + see; }
-
-    __device__ __forceinline__ int row_of(const Job& j, int c, int& head) const {
-        const int col = j.tile * kCols + c;
-        head = j.g * pl.shared + col % pl.shared;
-        return j.first + col / pl.shared;
-    }
-    // N results of one column from d0 on, and with `writes_rem` what is left of the stick
-    template <int N>
-    __device__ __forceinline__ void store(const Job& j, int c, int d0, const float (&x)[N], float sum, bool writes_rem) const {
-        int h;
-        const int t = row_of(j, c, h);
-        const T left = from_f32<T>(ex2(-sum));
-        T* o = (T*)p.o.ptr + h * p.o.stride_h + t * p.o.stride_t + d0;
-        const T* v = p.v.ptr ? (const T*)p.v.ptr + j.g * p.v.stride_h + t * p.v.stride_t + d0 : nullptr;
-        struct alignas(2 * sizeof(T)) Two {
-            T a, b;
-        };
-        if (N > 1 && pl.pairs) {
-            Two w[N / 2 + 1];
-            if (v)
-#pragma unroll
-                for (int i = 0; i + 1 < N; i += 2)
-                    if (d0 + i < p.head_dim) w[i / 2] = *(const Two*)(v + i);
-#pragma unroll
-            for (int i = 0; i + 1 < N; i += 2)
-                if (d0 + i < p.head_dim) {
-                    const float l = to_f32(left);
-                    *(Two*)(o + i) = v ? Two{from_f32<T>(fmaf(l, to_f32(w[i / 2].a), x[i])), from_f32<T>(fmaf(l, to_f32(w[i / 2].b), x[i + 1]))}
-                                       : Two{from_f32<T>(x[i]), from_f32<T>(x[i + 1])};
-                }
-        } else {
-#pragma unroll
-            for (int i = 0; i < N; ++i)
-                if (d0 + i < p.head_dim) o[i] = from_f32<T>(v ? fmaf(to_f32(left), to_f32(v[i]), x[i]) : x[i]);
-        }
-        if (writes_rem) ((T*)p.rem.ptr)[h * p.rem.stride_h + t * p.rem.stride_t] = left;
-    }
-};
-
-// One column of `count` partial results, from the right, joined by one warp: lane l has the values lane * N ... of x.  slot(a): the a-th one.
-// The loads do not wait for one another.
-template <int DP, int N, typename F>
-__device__ __forceinline__ void join_parts(int count, int c, int lane, F slot, float (&x)[N], float& sum) {
-    sum = 0.f;
-#pragma unroll
-    for (int i = 0; i < N; ++i) x[i] = 0.f;
-    for (int base = 0; base < count; base += 32) {
-        float s = base + lane < count ? slot(base + lane)[kCols * DP + c] : 0.f;
-#pragma unroll
-        for (int off = 1; off < 32; off <<= 1) {
-            const float y = __shfl_up_sync(0xffffffffu, s, off);
-            if (lane >= off) s += y;
-        }
-        float right = __shfl_up_sync(0xffffffffu, s, 1);
-        if (lane == 0) right = 0.f;
-        const float weight = ex2(-(sum + right));
-        const int n = min(32, count - base);
-#pragma unroll 8
-        for (int a = 0; a < n; ++a) {
-            const float w = __shfl_sync(0xffffffffu, weight, a);
-            const float* from = slot(base + a) + c * DP + lane * N;
-            alignas(16) float y[N];
-            if constexpr (N == 4) *(float4*)y = *(const float4*)from;
-            else if constexpr (N == 2) *(float2*)y = *(const float2*)from;
-            else y[0] = from[0];
-#pragma unroll
-            for (int i = 0; i < N; ++i) x[i] = fmaf(w, y[i], x[i]);
-        }
-        sum += __shfl_sync(0xffffffffu, s, 31);
-    }
-}
-
-template <typename T, int DP>
 __global__ void __launch_bounds__(32 * warps(DP), blocks_per_sm(DP))
 cached_kernel(const __grid_constant__ SbCacheParams p, const __grid_constant__ Plan pl, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
-    using K = Kernel<T, DP>;
-    constexpr int ST = K::ST, KW = K::KW, VW = K::VW, M = K::M, kWarps = warps(DP), kThreads = 32 * kWarps;
+    using K = Jobs<T, DP, kCols, 32>;
+    constexpr bool kSplitQ = sizeof(T) == 4;
+    constexpr int ST = stages(DP), KW = DP / 16, VW = DP / 32, M = DP / 16, kWarps = warps(DP), kThreads = 32 * kWarps;
     extern __shared__ uint8_t raw[];
     uint8_t* const sm = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);
-    __shared__ long long warp_sums[kWarps];
     __shared__ uint32_t gave_up;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rr = lane >> 2, cc = lane & 3;
     uint8_t* const ring = sm + (size_t)warp * ST * stage_bytes(DP);
     WarpScratch<ST>& ws = ((WarpScratch<ST>*)(sm + Layout<DP>::scratch))[warp];
     int* const starts = (int*)(sm + Layout<DP>::starts);
-    const int see = p.attend_current ? 1 : 0, P = p.page_tokens, R = p.requests;
+    const int see = p.attend_current ? 1 : 0, P = p.page_tokens;
     if (lane == 0)
         for (int s = 0; s < ST; ++s) mbar_init(&ws.full[s], 1);
     if (threadIdx.x == 0) gave_up = 0;
@@ -279,48 +114,12 @@ cached_kernel(const __grid_constant__ SbCacheParams p, const __grid_constant__ P
     pdl_wait();
     pdl_launch_dependents();
 
-    // where every request's units start: a prefix sum over the requests, by every block for itself
-    long long carry = 0;
-    bool bad = false;
-    for (int base = 0; base < R; base += kThreads) {
-        const int r = base + threadIdx.x;
-        long long mine = 0;
-        if (r < R) {
-            const int len = p.lengths[r];
-            int first = r, last = r + (len > 0 ? 1 : 0);
-            if (p.ends) {
-                first = r > 0 ? p.ends[r - 1] : 0;
-                last = p.ends[r];
-            }
-            const long long n = (long long)last - first;
-            if (first < 0 || n < 0 || last > p.tokens || len < n || len > (long long)p.width * P) bad = true;
-            else if (n > 0) mine = units_of(pl, len, (int)n, see);
-        }
-        long long x = mine;
-#pragma unroll
-        for (int off = 1; off < 32; off <<= 1) {
-            const long long y = __shfl_up_sync(0xffffffffu, x, off);
-            if (lane >= off) x += y;
-        }
-        if (lane == 31) warp_sums[warp] = x;
-        __syncthreads();
-        long long before = carry;
-        for (int w = 0; w < kWarps; ++w) {
-            if (w < warp) before += warp_sums[w];
-            carry += warp_sums[w];
-        }
-        if (r < R) starts[r] = (int)min(before + x - mine, 0x7fffffffll);
-        __syncthreads();
-    }
-    if (threadIdx.x == 0) starts[R] = (int)min(carry, 0x7fffffffll);
-    if (carry > 0x7fffffffll) bad = true, carry = 0;
-    if (bad) atomicOr(p.status, SBATTN_ST_BAD_SEQLENS);
-    __syncthreads();
+    const long long carry = scan_requests<K, kThreads>(p, pl, starts, see);
     const long long units = carry * p.kv_heads;
     // one share of the units per warp, neighbouring ones on different SMs; no warp waits for another from here on
     const long long shares = max(1ll, min((long long)gridDim.x * kWarps, units)), self = (long long)warp * gridDim.x + blockIdx.x;
     const long long w1 = min(units, units * (self + 1) / shares);
-    const K k{p, pl, starts, lane, see};
+    const K k{p, pl, starts, see};
     if (lane == 0) pl.seams[self] = make_int4(-1, 0, 0, 0);
 
     // ---- loads: the next step to load is ipos of a job (of request ir, head ig); lane l holds the pages and scales of the l-th step of a batch of 32
@@ -402,7 +201,7 @@ cached_kernel(const __grid_constant__ SbCacheParams p, const __grid_constant__ P
     const int pk = key_of_row<DP>(rr), place = place_of<DP>(lane);
     int pos = 0, end = 0, steps = 0, cols = 0, keys = 0, least = 0;
     bool packed = false;
-    uint32_t qh[2 * KW], ql[K::kSplitQ ? 2 * KW : 1];
+    uint32_t qh[2 * KW], ql[kSplitQ ? 2 * KW : 1];
     float acc[M][4];
     for (;;) {
         while (loaded < ST) {
@@ -467,7 +266,7 @@ cached_kernel(const __grid_constant__ SbCacheParams p, const __grid_constant__ P
                 const Four& f = nq[i >> 1];
                 const float a = to_f32(i & 1 ? f.c : f.a) * up, b = to_f32(i & 1 ? f.d : f.b) * up;
                 qh[i] = pack_f16(a, b);
-                if (K::kSplitQ) {
+                if (kSplitQ) {
                     const __half2 hi = *(const __half2*)&qh[i];
                     const float la = a - __low2float(hi), lb = b - __high2float(hi);  // NaN behind an infinity: the low term of that is zero
                     ql[i] = pack_f16(fabsf(a) <= 65504.f ? la : 0.f, fabsf(b) <= 65504.f ? lb : 0.f);
@@ -515,7 +314,7 @@ cached_kernel(const __grid_constant__ SbCacheParams p, const __grid_constant__ P
                     codes_to_f16(wa[w], a0, a2);
                     codes_to_f16(wb[w], a1, a3);
                     mma16816(s, a0, a1, a2, a3, qh[2 * w], qh[2 * w + 1]);
-                    if (K::kSplitQ) mma16816(s, a0, a1, a2, a3, ql[2 * w], ql[2 * w + 1]);
+                    if (kSplitQ) mma16816(s, a0, a1, a2, a3, ql[2 * w], ql[2 * w + 1]);
                 }
                 if (2 * cc < cols) {
                     float* const x0 = ws.x + 2 * cc * kColStride + ka;
@@ -671,7 +470,7 @@ cached_kernel(const __grid_constant__ SbCacheParams p, const __grid_constant__ P
             for (int m = 0; m < M; ++m)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) acc[m][i] += __shfl_xor_sync(0xffffffffu, acc[m][i], 2);
-        float* const slot = pl.slots + ((size_t)self * 2 + (starts_here ? 1 : 0)) * kSlot(DP);
+        float* const slot = pl.slots + ((size_t)self * 2 + (starts_here ? 1 : 0)) * slot_floats(kCols, DP);
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
             const int col = 2 * cc + c, d0 = rr * 4 * VW;
@@ -708,57 +507,7 @@ cached_kernel(const __grid_constant__ SbCacheParams p, const __grid_constant__ P
         }
     }
 
-    // rem of the rows that belong to no request
-    if (p.ends) {
-        const int first = R > 0 ? max(0, p.ends[R - 1]) : 0;
-        const long long rows = (long long)max(0, p.tokens - first) * p.heads;
-        for (long long i = (long long)blockIdx.x * kThreads + threadIdx.x; i < rows; i += (long long)gridDim.x * kThreads)
-            ((T*)p.rem.ptr)[(i % p.heads) * p.rem.stride_h + (first + i / p.heads) * p.rem.stride_t] = from_f32<T>(0.f);
-    } else {
-        for (int t = blockIdx.x * kThreads + threadIdx.x; t < p.tokens; t += gridDim.x * kThreads)
-            if (t >= R || p.lengths[t] <= 0)
-                for (int h = 0; h < p.heads; ++h) ((T*)p.rem.ptr)[h * p.rem.stride_h + t * p.rem.stride_t] = from_f32<T>(0.f);
-    }
-}
-
-// Jobs that several shares have parts of.  One block per seam between two shares: its warps take the columns, and where there are few of them, parts
-// of the line of partial results, which meet in shared memory.
-template <typename T, int DP>
-__global__ void __launch_bounds__(32 * kCols) cached_join_kernel(const __grid_constant__ SbCacheParams p, const __grid_constant__ Plan pl) {
-    using K = Kernel<T, DP>;
-    constexpr int N = DP / 32;
-    __shared__ float xs[kCols][DP], sums[kCols];
-    pdl_wait();
-    pdl_launch_dependents();
-    const int b = blockIdx.x + 1, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int4 seam = pl.seams[b];
-    if (seam.x < 0) return;
-    const K k{p, pl, nullptr, lane, p.attend_current ? 1 : 0};
-    Job j;
-    j.r = seam.x;
-    j.g = seam.y;
-    j.tile = seam.z;
-    k.request(j.r, j.first, j.n, j.len);
-    j.cols = min(kCols, j.n * pl.shared - j.tile * kCols);
-    const int count = seam.w - b + 2, splits = j.cols <= 1 ? 8 : j.cols <= 2 ? 4 : j.cols <= 4 ? 2 : 1;
-    const int c = warp / splits, part = warp % splits, a0 = count * part / splits, a1 = count * (part + 1) / splits;
-    float x[N], sum = 0.f;
-    if (c < j.cols)
-        join_parts<DP>(a1 - a0, c, lane, [&](int a) { return pl.slots + ((size_t)(b - 1 + a0 + a) * 2 + (a0 + a == 0 ? 1 : 0)) * kSlot(DP); }, x, sum);
-    if (splits > 1) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) xs[warp][lane * N + i] = x[i];
-        if (lane == 0) sums[warp] = sum;
-        __syncthreads();
-        if (part != 0) return;
-        for (int s = 1; s < splits; ++s) {
-            const float weight = ex2(-sum);
-#pragma unroll
-            for (int i = 0; i < N; ++i) x[i] = fmaf(weight, xs[warp + s][lane * N + i], x[i]);
-            sum += sums[warp + s];
-        }
-    }
-    if (c < j.cols) k.store(j, c, lane * N, x, sum, lane == 0);
+    clear_rem<T>(p, kThreads);
 }
 
 int64_t grid_of(const SbCacheParams& p) {
@@ -768,24 +517,10 @@ int64_t grid_of(const SbCacheParams& p) {
     return most < all ? (most < 1 ? 1 : most) : all;
 }
 
-Plan plan_of(const SbCacheParams& p, int64_t grid) {
-    Plan pl;
-    pl.shared = p.heads / p.kv_heads;
-    const int64_t size = p.dtype == SBATTN_F32 ? 4 : 2;
-    const auto even = [&](const SbMat& m, int n) { return (((uintptr_t)m.ptr | (uintptr_t)(m.stride_h * size) | (uintptr_t)(m.stride_t * size)) & (n * size - 1)) == 0; };
-    pl.quads = p.head_dim % 4 == 0 && even(p.q, 4);
-    pl.pairs = p.head_dim % 2 == 0 && even(p.o, 2) && even(p.v, 2);
-    pl.warps = (int)grid * warps(p.row);
-    char* w = (char*)p.workspace;
-    pl.seams = (int4*)w;
-    pl.slots = (float*)(w + align_up(16 * (size_t)pl.warps, 256));
-    return pl;
-}
-
 template <typename T, int DP>
 int launch(const SbCacheParams& p, cudaStream_t st) {
     const int64_t grid = grid_of(p);
-    const Plan pl = plan_of(p, grid);
+    const Plan pl = make_plan(p, (int)grid * warps(DP));
     CUtensorMap km, vm;
     const int box = p.page_tokens < 32 ? p.page_tokens : 32;
     if (encode_page_map(&km, p.k_codes, DP, (int64_t)p.kv_heads * p.page_tokens, p.pages, p.k_stride, box) != 0 ||
@@ -795,7 +530,7 @@ int launch(const SbCacheParams& p, cudaStream_t st) {
     if (rc != 0) return rc;
     rc = launch_kernel(cached_kernel<T, DP>, dim3((unsigned)grid), dim3(32 * warps(DP)), Layout<DP>::bytes(p.requests), st, p, pl, km, vm);
     if (rc != 0) return rc;
-    return launch_kernel(cached_join_kernel<T, DP>, dim3((unsigned)pl.warps - 1), dim3(32 * kCols), 0, st, p, pl);
+    return launch_join<T, DP, kCols>(p, pl, st);
 }
 
 template <typename T>
@@ -805,13 +540,20 @@ int launch_row(const SbCacheParams& p, cudaStream_t st) {
 
 }  // namespace
 
+// Many queries per key: the kernel of sb_cached_tc.cu
+static bool many_queries(const SbCacheParams& p) {
+    const int64_t shared = p.heads / p.kv_heads;
+    return p.dtype == SBATTN_BF16 && p.row >= 64 && p.ends && p.requests > 0 && (int64_t)p.tokens * shared >= 64 * (int64_t)p.requests;
+}
+
 size_t cached_workspace(const SbCacheParams& p) {
     if (p.heads == 0 || p.kv_heads == 0) return 0;
-    const size_t n = (size_t)grid_of(p) * warps(p.row);
-    return align_up(16 * n, 256) + n * 2 * kSlot(p.row) * sizeof(float);
+    if (many_queries(p)) return cached_tc_workspace(p);
+    return plan_bytes(grid_of(p) * warps(p.row), kCols, p.row);
 }
 
 int launch_cached_fwd(const SbCacheParams& p, cudaStream_t st) {
+    if (many_queries(p)) return launch_cached_tc(p, st);
     if (p.dtype == SBATTN_F32) return launch_row<float>(p, st);
     if (p.dtype == SBATTN_F16) return launch_row<__half>(p, st);
     return launch_row<__nv_bfloat16>(p, st);

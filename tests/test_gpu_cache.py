@@ -283,7 +283,7 @@ class Problem:
         from stickbreaking_attention_b200 import sb_attn_cached
         return sb_attn_cached(self.q, self.cache, ints(self.tables).reshape(len(self.lengths), -1), ints(self.lengths), ints(np.cumsum(self.new)) if ends else None, **kw)
 
-    def want(self, inv_temp=None, attend_current=False, v=None):
+    def want(self, inv_temp=None, attend_current=False, v=None, wide=False):
         """o, rem and their bounds without the rounding to the output's type."""
         inv_temp = self.dim ** -0.5 if inv_temp is None else inv_temp
         q = self.q.double().cpu().numpy()
@@ -293,16 +293,16 @@ class Problem:
             rows = slice(at, at + n)
             at += n
             per = [orc.attend(q[h, rows], self.k[r][h * self.kv // self.heads], self.v[r][h * self.kv // self.heads], n, inv_temp, attend_current,
-                              own[h * self.kv // self.heads, rows] if own is not None else None) for h in range(self.heads)]
+                              own[h * self.kv // self.heads, rows] if own is not None else None, wide) for h in range(self.heads)]
             for out, x in zip(outs, zip(*per)):
                 out.append(np.stack(x))
         return [np.concatenate(x, 1) for x in outs]
 
-    def check(self, ends=True, v=None, **kw):
+    def check(self, ends=True, v=None, wide=False, **kw):
         o, rem = self.run(ends, v=v, **kw)
         rows = sum(self.new)
         assert o.shape == self.q.shape and rem.shape == self.q.shape[:2] and o.dtype == rem.dtype == self.q.dtype
-        self.compare(o[:, :rows], rem[:, :rows], *self.want(v=v, **kw), own_v=v)
+        self.compare(o[:, :rows], rem[:, :rows], *self.want(v=v, wide=wide, **kw), own_v=v)
         assert (rem[:, rows:] == 0).all()
         return o, rem
 
@@ -342,8 +342,86 @@ def test_shared_heads(shared, dim):
 def test_several_new_tokens(dtype, shared, current, dim):
     lengths, new = [40, 1, 9, 100, 33, 300, 64, 5], [3, 1, 9, 17, 0, 70, 64, 2]
     p = Problem(lengths, new, heads=2 * shared, kv=2, dim=dim, page=16, dtype=dtype, lean=2.0, seed=1, extra_rows=5)
-    p.check(attend_current=current)
-    p.check(attend_current=current, v=p.own_v)
+    wide = dtype == "bf16" and shared == 3  # enough queries for the kernel that takes 256 at a time
+    p.check(attend_current=current, wide=wide)
+    p.check(attend_current=current, v=p.own_v, wide=wide)
+
+
+@pytest.mark.parametrize("dim, page", [(128, 64), (64, 16), (100, 32), (48, 128), (128, 16), (64, 64)])
+@pytest.mark.parametrize("shared, lengths, new", [(1, [200], [100]), (4, [70, 1000, 300], [70, 100, 41]), (1, [700, 64, 129], [300, 64, 128]), (8, [333], [33]), (3, [2500], [90])])
+@pytest.mark.parametrize("current", [False, True])
+def test_many_queries(dim, page, shared, lengths, new, current):
+    """Tiles of 256 queries, full and not, one half of them empty, sequences of one step and of many, cut into shares."""
+    p = Problem(lengths, new, heads=2 * shared, kv=2, dim=dim, page=page, dtype="bf16", lean=3.0, seed=dim + shared, extra_rows=3)
+    p.check(attend_current=current, v=p.own_v, wide=True)
+    p.check(attend_current=current, wide=True)
+
+
+def test_many_queries_many_requests():
+    rng = np.random.default_rng(1)
+    lengths = [int(x) for x in rng.integers(0, 400, 90)]
+    new = [min(t, int(n)) for t, n in zip(lengths, rng.integers(0, 260, 90))]
+    Problem(lengths, new, heads=2, kv=1, dim=64, page=32, dtype="bf16", lean=2.0).check(wide=True)
+
+
+@pytest.mark.parametrize("case", ["far", "strong", "hot", "scaled"])
+def test_many_queries_extreme_logits(case):
+    p = Problem([300, 150], [100, 90], heads=2, dim=64, page=16, dtype="bf16", lean=0.0, seed=3)
+    if case == "far":
+        p.q = torch.full_like(p.q, -1.0)
+        for r, t in enumerate(p.lengths):
+            p.k[r][:] = 0.625
+            for b in range(-(-t // 16)):
+                p.cache.k.view(torch.uint8)[p.tables[r, b], :, :min(16, t - 16 * b)] = int(orc.to_code(np.float64(0.625)))
+                p.cache.k_scale[p.tables[r, b]] = 1.0
+    p.check(inv_temp={"far": 1.0, "strong": 4.0, "hot": 30.0, "scaled": 0.0}[case], wide=True)
+
+
+def test_many_queries_strides():
+    p = Problem([170, 133], [100, 60], heads=4, kv=2, dim=128, page=32, dtype="bf16", halves=True, lean=1.0)
+    flat = p.run(v=p.own_v)
+    p.q = p.q.permute(1, 0, 2).contiguous().permute(1, 0, 2)
+    major = p.check(v=p.own_v.permute(1, 0, 2).contiguous().permute(1, 0, 2), wide=True)
+    assert all(torch.equal(a, b) for a, b in zip(flat, major))
+    odd = torch.zeros(4, p.q.shape[1], 131, device="cuda", dtype=torch.bfloat16)
+    odd[..., 1:129] = p.q
+    p.q = odd[..., 1:129]  # rows that do not start at an aligned address
+    assert all(torch.equal(a, b) for a, b in zip(flat, p.run(v=p.own_v)))
+
+
+def test_many_queries_nan():
+    """NaN in a value that some queries of a tile see; in a key; in a value that all see."""
+    p = Problem([350, 200], [100, 70], heads=2, dim=64, page=16, dtype="bf16", lean=1.0)
+    clean_o, clean_rem = p.run()
+    for key in (300, 20):  # rows 0 ... 99 are the tokens 250 ... 349
+        page, place, sees = p.tables[0, key // 16], key % 16, max(0, key + 1 - 250)
+        codes = p.cache.v.view(torch.uint8)
+        was = int(codes[page, 1, place, 9])
+        codes[page, 1, place, 9] = 255
+        o, rem = p.run()
+        bad = torch.zeros_like(o, dtype=torch.bool)
+        bad[1, sees:100, 9] = True
+        assert o[bad].isnan().all() and torch.equal(o[~bad], clean_o[~bad]) and torch.equal(rem, clean_rem)
+        codes[page, 1, place, 9] = was
+    page, place = p.tables[0, 300 // 16], 300 % 16
+    p.cache.k.view(torch.uint8)[page, 0, place, 3] = 127
+    o, rem = p.run()
+    bad = torch.zeros_like(o, dtype=torch.bool)
+    bad[0, 51:100] = True
+    assert o[bad].isnan().all() and not o[~bad].isnan().any() and rem[0, 51:100].isnan().all() and int(rem.isnan().sum()) == 49
+
+
+@pytest.mark.parametrize("page_index", [-1, 10 ** 6])
+def test_many_queries_bad_pages(page_index, monkeypatch):
+    from stickbreaking_attention_b200 import check_status
+    monkeypatch.setenv("SBATTN_CHECK_STATUS", "0")
+    p = Problem([350, 200], [100, 70], heads=2, dim=64, page=16, dtype="bf16")
+    good = p.run()
+    p.tables[0, 3] = page_index
+    o, rem = p.run()
+    with pytest.raises(ValueError, match="page index"):
+        check_status()
+    assert torch.equal(o[:, 100:], good[0][:, 100:]) and torch.equal(rem[:, 100:], good[1][:, 100:])
 
 
 @pytest.mark.parametrize("lean", [0.0, 3.0, 8.0])
