@@ -523,8 +523,8 @@ int launch(const SbCacheParams& p, cudaStream_t st) {
     const Plan pl = make_plan(p, (int)grid * warps(DP));
     CUtensorMap km, vm;
     const int box = p.page_tokens < 32 ? p.page_tokens : 32;
-    if (encode_page_map(&km, p.k_codes, DP, (int64_t)p.kv_heads * p.page_tokens, p.pages, p.k_stride, box) != 0 ||
-        encode_page_map(&vm, p.v_codes, DP, (int64_t)p.kv_heads * p.page_tokens, p.pages, p.v_stride, box) != 0)
+    if (encode_page_map(&km, p.k_codes, DP, (int64_t)p.kv_heads * p.page_tokens, p.pages, p.k_stride, box, true) != 0 ||
+        encode_page_map(&vm, p.v_codes, DP, (int64_t)p.kv_heads * p.page_tokens, p.pages, p.v_stride, box, true) != 0)
         return kMapEncodeFailed;
     int rc = ensure_kernel_attrs((const void*)cached_kernel<T, DP>, (int)Layout<DP>::bytes(SBATTN_MAX_REQUESTS), true);
     if (rc != 0) return rc;

@@ -120,7 +120,21 @@ struct Jobs {
         struct alignas(2 * sizeof(T)) Two {
             T a, b;
         };
-        if (N > 1 && pl.pairs) {
+        struct alignas(sizeof(T) == 2 ? 16 : 32) Eight {
+            T a[8];
+        };
+        if (N % 8 == 0 && sizeof(T) == 2 && pl.octets) {
+#pragma unroll
+            for (int i = 0; i + 7 < N; i += 8)
+                if (d0 + i < p.head_dim) {
+                    const float l = to_f32(left);
+                    Eight w, y;
+                    if (v) w = *(const Eight*)(v + i);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) y.a[e] = from_f32<T>(v ? fmaf(l, to_f32(w.a[e]), x[i + e]) : x[i + e]);
+                    *(Eight*)(o + i) = y;
+                }
+        } else if (N > 1 && pl.pairs) {
             Two w[N / 2 + 1];
             if (v)
 #pragma unroll

@@ -11,7 +11,8 @@
 // the weight of key m is e_m (product of d to its left in the group) W / (product of d of the group): one reciprocal per four keys.
 // x is clamped at 30 (1 - beta = 2^-30), so that the product of a group stays below 2^121.
 //
-// Warps of a block (416 threads): 0-3 / 4-7 row warps of the first / second half, 8-11 load codes and queries and convert them, 12 issues tcgen05.mma.
+// Warps of a block (512 threads, 128 registers): 0-3 / 4-7 row warps of the first / second half, 8-11 / 12-14 convert the codes of the values / keys, which
+// TMA brings to shared memory a step ahead, all of them the queries, 15 issues tcgen05.mma.
 // Tensor memory (512 columns): scores of the halves at 0 / 128 (weights overwrite the right half of their scores), sums at 256 / 384.
 #include "sb_cached.cuh"
 #include "sb_tc_common.cuh"
@@ -24,37 +25,36 @@ using namespace sm100;
 using namespace cached;
 using bf16 = __nv_bfloat16;
 
-constexpr int kThreads = 416, kConverters = 128, kMmaWarp = 12;
+constexpr int kThreads = 512, kMmaWarp = 15, kConverters = 7, kValueWarps = 4;
 constexpr int kTile = 256, kStep = 128;  // queries of a tile, keys of a step
 constexpr uint32_t kTmemCols = 512, kColS = 0, kColO = 256, kColP = 64;
 constexpr int kScaleSlots = 4;
-enum Bar { Q_FULL0, Q_FULL1, Q_EMPTY, K_FULL0, K_FULL1, K_EMPTY0, K_EMPTY1, V_FULL0, V_FULL1, V_EMPTY0, V_EMPTY1, SC_FULL0, SC_FULL1, SC_FULL2, SC_FULL3,
+enum Bar { Q_FULL0, Q_FULL1, Q_EMPTY, K_FULL, K_EMPTY, RAW_K, RAW_V, READ_K, READ_V, V_FULL0, V_FULL1, V_EMPTY0, V_EMPTY1, SC_FULL0, SC_FULL1, SC_FULL2, SC_FULL3,
            S_READY0, S_READY1, P_READY0, P_READY1, O_READY0, O_READY1, O_FREE0, O_FREE1, kNumBars };
 
 struct Small {  // behind the tiles
     uint64_t bars[kNumBars];
     float temp[2][kTile];            // of the jobs in turn: inv_temp log2(e) by what the query was multiplied with
     float ks[kScaleSlots][8], vs[kScaleSlots][8];  // of the steps in turn: scales of 16 keys each
-    uint32_t nan_job[2];             // 1 + number of the job that has NaN among the values of keys that not all of its queries see
+    uint32_t nan_job[4];             // of the jobs in turn: 1 + number of the job, if it has NaN among the values of keys that not all of its queries see
     uint32_t tmem, abort;
 };
 
-// one chunk of 32 keys: weights relative to an entering W of 1, and the products of 1 + e of the eight groups of four
+// 16 keys: weights relative to an entering W of 1, and the products of 1 + e of the four groups of four; groups in pairs, one packed instruction for both
 template <bool kMasked>
-__device__ __forceinline__ void sweep(const uint32_t (&s)[32], float scale0, float scale1, int col0, int lim, float2 (&p)[4][4], float2 (&run)[4]) {
+__device__ __forceinline__ void sweep(const uint32_t (&s)[16], float scale, int col0, int lim, float2 (&p)[2][4], float2 (&run)[2]) {
     const auto e_of = [](float x) {
         asm("min.NaN.f32 %0, %0, %1;" : "+f"(x) : "f"(30.f));
         return ex2_approx(x);
     };
 #pragma unroll
-    for (int h = 0; h < 4; ++h) {
-        const float sc = h < 2 ? scale0 : scale1;
+    for (int h = 0; h < 2; ++h) {
         run[h] = make_float2(1.f, 1.f);
 #pragma unroll
         for (int m = 0; m < 4; m += 2) {
             const int i0 = 8 * h + m, i1 = i0 + 4;
-            const float2 x0 = __fmul2_rn(make_float2(__uint_as_float(s[i0]), __uint_as_float(s[i0 + 1])), make_float2(sc, sc));
-            const float2 x1 = __fmul2_rn(make_float2(__uint_as_float(s[i1]), __uint_as_float(s[i1 + 1])), make_float2(sc, sc));
+            const float2 x0 = __fmul2_rn(make_float2(__uint_as_float(s[i0]), __uint_as_float(s[i0 + 1])), make_float2(scale, scale));
+            const float2 x1 = __fmul2_rn(make_float2(__uint_as_float(s[i1]), __uint_as_float(s[i1 + 1])), make_float2(scale, scale));
             float2 ea = make_float2(e_of(x0.x), e_of(x1.x)), eb = make_float2(e_of(x0.y), e_of(x1.y));
             if (kMasked) {
                 if (col0 + i0 >= lim) ea.x = 0.f;
@@ -69,49 +69,90 @@ __device__ __forceinline__ void sweep(const uint32_t (&s)[32], float scale0, flo
         }
     }
 }
-// from right to left: the factor of every group; W <- what leaves the chunk on its left
-__device__ __forceinline__ void carries(const float2 (&run)[4], float& W, float2 (&f)[4]) {
+// from right to left: the factor of every group; W <- what leaves the 16 keys on their left
+__device__ __forceinline__ void carries(const float2 (&run)[2], float& W, float2 (&f)[2]) {
 #pragma unroll
-    for (int h = 3; h >= 0; --h) {
+    for (int h = 1; h >= 0; --h) {
         f[h].y = W * rcp_approx(run[h].y);
         f[h].x = f[h].y * rcp_approx(run[h].x);
         W = f[h].x;
     }
 }
-__device__ __forceinline__ void finish(const float2 (&p)[4][4], const float2 (&f)[4], float vs0, float vs1, uint32_t (&w)[16]) {
+__device__ __forceinline__ void finish(const float2 (&p)[2][4], const float2 (&f)[2], float vs, uint32_t (&w)[8]) {
+    const float2 v = make_float2(vs, vs);  // not into f, which may be as small as 2^-120
 #pragma unroll
-    for (int h = 0; h < 4; ++h) {
-        const float2 v = h < 2 ? make_float2(vs0, vs0) : make_float2(vs1, vs1);  // not into f, which may be as small as 2^-120
+    for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int m = 0; m < 4; m += 2) {
             const float2 a = __fmul2_rn(__fmul2_rn(p[h][m], f[h]), v), b = __fmul2_rn(__fmul2_rn(p[h][m + 1], f[h]), v);
             w[4 * h + m / 2] = pack_bf16(a.x, b.x);
             w[4 * h + 2 + m / 2] = pack_bf16(a.y, b.y);
         }
+}
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]),
+                 "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                 : "memory");
+}
+
+// One row of a step, 32 keys at a time from the right: the scores of the next 32 travel while the weights of these are finished.  Weights go to columns of
+// scores that have been read.  A loop, not its four rounds one behind the other: the code of all roles has to stay in the instruction cache (12 % of the kernel).
+template <bool kMasked>
+__device__ __forceinline__ void row_step(uint32_t s_base, const float* ks, const float* vs, float temp, int key0, int lim, float& W) {
+    uint32_t u[2][16], w[8];
+    float2 pw[2][2][4], run[2][2], f[2][2];
+    tmem_ld16(s_base + 96, u[0]);
+    tmem_ld16(s_base + 112, u[1]);
+    tmem_wait_ld(u[0]);
+    tmem_wait_ld(u[1]);
+#pragma unroll 1
+    for (int ch = 6; ch >= 0; ch -= 2) {
+        sweep<kMasked>(u[1], ks[ch + 1] * temp, key0 + 16 * ch + 16, lim, pw[1], run[1]);
+        sweep<kMasked>(u[0], ks[ch] * temp, key0 + 16 * ch, lim, pw[0], run[0]);
+        if (ch > 0) {
+            tmem_ld16(s_base + 16 * (ch - 2), u[0]);
+            tmem_ld16(s_base + 16 * (ch - 1), u[1]);
+        }
+        carries(run[1], W, f[1]);
+        carries(run[0], W, f[0]);
+        finish(pw[1], f[1], vs[ch + 1], w);
+        tmem_st8(s_base + kColP + 8 * (ch + 1), w);
+        finish(pw[0], f[0], vs[ch], w);
+        tmem_st8(s_base + kColP + 8 * ch, w);
+        if (ch > 0) {
+            tmem_wait_ld(u[0]);
+            tmem_wait_ld(u[1]);
+        }
     }
 }
 
 template <int DP>
-__global__ void __launch_bounds__(kThreads, 1) cached_tc_kernel(const __grid_constant__ SbCacheParams p, const __grid_constant__ Plan pl) {
+__global__ void __launch_bounds__(kThreads, 1) cached_tc_kernel(const __grid_constant__ SbCacheParams p, const __grid_constant__ Plan pl, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
     using J = Jobs<bf16, DP, kTile, kStep>;
     constexpr int kHalfBytes = 128 * DP * 2, kBoxBytes = 128 * 128;
     extern __shared__ __align__(1024) uint8_t smem[];
     uint8_t* const sQ = smem;                       // two halves
-    uint8_t* const sK = sQ + 2 * kHalfBytes;        // two stages
-    uint8_t* const sV = sK + 2 * kHalfBytes;
-    Small& sm = *(Small*)(sV + 2 * kHalfBytes);
+    uint8_t* const sK = sQ + 2 * kHalfBytes;        // one stage: it is free as soon as both halves have their scores
+    uint8_t* const sV = sK + kHalfBytes;            // two stages
+    uint8_t* const raw_k = sV + 2 * kHalfBytes;     // codes of a step
+    uint8_t* const raw_v = raw_k + kStep * DP;
+    Small& sm = *(Small*)(raw_v + kStep * DP);
     int* const starts = (int*)(&sm + 1);
     volatile uint32_t* const abort_flag = &sm.abort;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, see = p.attend_current ? 1 : 0, P = p.page_tokens;
     if (tid == 0) {
         for (int i = 0; i < kNumBars; ++i) {
-            const bool by_converters = i == Q_FULL0 || i == Q_FULL1 || i == K_FULL0 || i == K_FULL1 || i == V_FULL0 || i == V_FULL1;
+            const bool by_all = i == Q_FULL0 || i == Q_FULL1, by_values = i == V_FULL0 || i == V_FULL1 || i == READ_V;
             const bool by_rows = i == P_READY0 || i == P_READY1 || i == O_FREE0 || i == O_FREE1;
-            mbar_init(&sm.bars[i], by_converters ? kConverters : by_rows ? 128 : i >= SC_FULL0 && i <= SC_FULL3 ? 4 : 1);
+            mbar_init(&sm.bars[i], by_all ? 32 * kConverters : i == K_FULL || i == READ_K ? 32 * (kConverters - kValueWarps) : by_values ? 32 * kValueWarps : by_rows ? 128 : i >= SC_FULL0 && i <= SC_FULL3 ? 2 : 1);
         }
-        sm.nan_job[0] = sm.nan_job[1] = 0;
+        for (int i = 0; i < 4; ++i) sm.nan_job[i] = 0;
         sm.abort = (smem_u32(smem) & 1023u) ? 1u : 0u;  // the swizzled tiles need a 1024-byte aligned base
         fence_barrier_init();
+    }
+    if (tid == 0) {
+        tma_prefetch_desc(&kmap);
+        tma_prefetch_desc(&vmap);
     }
     if (warp == kMmaWarp) {
         tmem_alloc(&sm.tmem, kTmemCols);
@@ -133,17 +174,18 @@ __global__ void __launch_bounds__(kThreads, 1) cached_tc_kernel(const __grid_con
 
     if (warp >= 8 && warp < kMmaWarp) {
         // ------------------------------------------------------------------ codes and queries to operands
-        constexpr int kPasses = DP / 16, kPerRow = DP / 16;  // 16-byte loads of a step and lane, for keys and for values; of a row
-        const int cw = warp - 8, ct = tid - 256;
-        const int chunk = lane % kPerRow, row0 = 32 * cw + lane / kPerRow, dr = 32 / kPerRow;  // rows row0 + dr i
+        const bool values = warp < 8 + kValueWarps;
+        const int group = values ? kValueWarps : kConverters - kValueWarps, gw = values ? warp - 8 : warp - 8 - kValueWarps;
+        constexpr int kPerRow = DP / 16, kRowsALoad = 32 / kPerRow;  // 16-byte pieces of a row; rows a warp takes at a time
+        const int chunk = lane % kPerRow, row0 = lane / kPerRow;
         const int flip = DP == 128 ? (chunk >> 2) & 1 : 0;  // which half of 16 values is stored first: all banks once
-        const auto place = [&](int row, int half) {  // 8 values (16 bytes) of a row: [128 rows][64 values] boxes, 128-byte swizzle
-            const int c16 = 2 * chunk + half;
-            return (c16 >> 3) * kBoxBytes + row * 128 + (((c16 & 7) ^ (row & 7)) << 4);
-        };
-        uint4 kx[kPasses], vx[kPasses];
-        float sk[2], sv[2];
-        uint32_t ph_ke = 3, ph_ve = 3, ph_qe = 1, step = 0, jobs = 0;
+        const CUtensorMap* const map = values ? &vmap : &kmap;
+        uint64_t* const raw_full = &sm.bars[values ? RAW_V : RAW_K];
+        uint8_t* const raw = values ? raw_v : raw_k;
+        const float* const scales = values ? p.v_scale : p.k_scale;
+        const int64_t scale_stride = values ? p.v_scale_stride : p.k_scale_stride;
+        const int box = min(P, kStep), nb = kStep / box;  // keys of a load, loads of a step
+        uint32_t ph_e = 3, ph_qe = 1, step = 0, jobs = 0, issued = 0;
         bool ok = true;
         for (long long u = u0; u < u1 && ok;) {
             const Job j = k.open(u, u1, r0);
@@ -151,154 +193,121 @@ __global__ void __launch_bounds__(kThreads, 1) cached_tc_kernel(const __grid_con
             const int first = k.first_pos(j);
             if (first >= j.end) continue;
             const int least = k.sees(j, 0);
-            const int* const table = p.tables + j.r * p.table_stride;
-            const auto load = [&](int pos) {
-                const int key0 = kStep * (j.steps - 1 - pos);
-                int page[2];
-#pragma unroll
-                for (int g = 0; g < 2; ++g) {  // this warp's 32 keys lie in one page, or in two of 16 tokens
-                    const int key = key0 + 32 * cw + 16 * g;
-                    page[g] = 0;
-                    sk[g] = sv[g] = 0.f;
-                    if (key >= j.keys) continue;
-                    page[g] = table[key / P];
-                    if (page[g] < 0 || page[g] >= p.pages) {
-                        if (lane == 0) atomicOr(p.status, SBATTN_ST_BAD_PAGES);
-                        page[g] = 0;
+            int page = 0, batch = first;  // of the group's first warp, lane l: page and scale of load l % nb of step l / nb of a batch of 32 / nb
+            float scale = 0.f;
+            const auto load = [&](int pos) {  // by the group's first warp, when the whole group has read the codes before
+                if (gw != 0) return;
+                if (pos == batch) {
+                    const int s = lane / nb, key = kStep * (j.steps - 1 - (pos + s)) + box * (lane % nb);
+                    page = 0;
+                    scale = 0.f;
+                    if (pos + s < j.end && key < j.keys) {
+                        page = p.tables[j.r * p.table_stride + key / P];
+                        if (page < 0 || page >= p.pages) {
+                            atomicOr(p.status, SBATTN_ST_BAD_PAGES);
+                            page = 0;
+                        }
+                        scale = scales[page * scale_stride + j.g];
                     }
-                    sk[g] = p.k_scale[page[g] * p.k_scale_stride + j.g];
-                    sv[g] = p.v_scale[page[g] * p.v_scale_stride + j.g];
+                    batch += 32 / nb;
                 }
-#pragma unroll
-                for (int i = 0; i < kPasses; ++i) {
-                    const int row = row0 + dr * i, key = key0 + row;
-                    kx[i] = vx[i] = make_uint4(0u, 0u, 0u, 0u);
-                    if (key < j.keys) {
-                        const int64_t at = ((int64_t)j.g * P + key % P) * DP + 16 * chunk, pg = (row & 16) ? page[1] : page[0];
-                        kx[i] = *(const uint4*)((const uint8_t*)p.k_codes + pg * p.k_stride + at);
-                        vx[i] = *(const uint4*)((const uint8_t*)p.v_codes + pg * p.v_stride + at);
-                    }
+                const int l0 = nb * (pos - (batch - 32 / nb)), i = lane - l0, key0 = kStep * (j.steps - 1 - pos), key = key0 + box * i;
+                if (i == 0) mbar_expect_tx(raw_full, min(nb, (j.keys - key0 + box - 1) / box) * box * DP);
+                __syncwarp();
+                if (i >= 0 && i < nb) {
+                    if (key < j.keys) tma_load_3d(raw + box * i * DP, map, raw_full, 0, j.g * P + key % P, page);
+                    float* const to = (values ? sm.vs : sm.ks)[issued % kScaleSlots] + i * (box / 16);
+                    for (int e = 0; e < box / 16; ++e) to[e] = scale;
                 }
+                __syncwarp();
+                if (i == 0) mbar_arrive(&sm.bars[SC_FULL0 + issued % kScaleSlots]);
+                ++issued;
             };
             load(first);
-            // the queries, when the last product with the ones before is done
+            // the queries, when the last product with the ones before is done: 16 bytes a lane
             ok = mbar_wait(&sm.bars[Q_EMPTY], ph_qe & 1, abort_flag);
             ph_qe ^= 1;
             if (!ok) break;
-            for (int c = ct; c < kTile; c += kConverters) {
+            constexpr int kLanes = DP / 8, kRows = 32 / kLanes;  // lanes of a row, rows of a load
+#pragma unroll 6
+            for (int c = (warp - 8) * kRows + lane / kLanes; c < kTile; c += kConverters * kRows) {
+                const int d = 8 * (lane % kLanes);
                 int h = 0, t = 0;
                 if (c < j.cols) t = k.row_of(j, c, h);
-                const bf16* q = (const bf16*)p.q.ptr + h * p.q.stride_h + t * p.q.stride_t;
-                const auto eight = [&](int d, uint32_t (&w)[4]) {
-                    w[0] = w[1] = w[2] = w[3] = 0u;
-                    if (c >= j.cols) return;
+                const bf16* q = (const bf16*)p.q.ptr + h * p.q.stride_h + t * p.q.stride_t + d;
+                alignas(16) uint32_t w[4] = {0u, 0u, 0u, 0u};
+                if (c < j.cols) {
                     if (pl.octets) {
-                        if (d < p.head_dim) {
-                            const uint4 x = *(const uint4*)(q + d);
-                            w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w;
-                        }
+                        if (d < p.head_dim) *(uint4*)w = *(const uint4*)q;
                     } else {
 #pragma unroll
                         for (int i = 0; i < 8; ++i)
-                            if (d + i < p.head_dim) w[i >> 1] |= (uint32_t)__bfloat16_as_ushort(q[d + i]) << (16 * (i & 1));
-                    }
-                };
-                const auto lo = [](uint32_t w) { return __uint_as_float(w << 16); };
-                const auto hi = [](uint32_t w) { return __uint_as_float(w & 0xffff0000u); };
-                float top = 0.f;
-#pragma unroll 4
-                for (int d = 0; d < DP; d += 8) {
-                    uint32_t w[4];
-                    eight(d, w);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float a = fabsf(lo(w[i])), b = fabsf(hi(w[i]));
-                        if (a <= 3.4028234664e38f) top = fmaxf(top, a);
-                        if (b <= 3.4028234664e38f) top = fmaxf(top, b);
+                            if (d + i < p.head_dim) w[i >> 1] |= (uint32_t)__bfloat16_as_ushort(q[i]) << (16 * (i & 1));
                     }
                 }
+                float y[8], top = 0.f;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    y[i] = __uint_as_float(i & 1 ? w[i >> 1] & 0xffff0000u : w[i >> 1] << 16);
+                    const float a = fabsf(y[i]);
+                    if (a <= 3.4028234664e38f) top = fmaxf(top, a);
+                }
+#pragma unroll
+                for (int off = 1; off < kLanes; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
                 const int e = top > 0.f ? max((int)(__float_as_uint(top) >> 23) - 127, -112) : 14;  // up to 2^(e + 1)
                 const float up = pow2(14 - e);
-                uint8_t* const dst = sQ + (c >> 7) * kHalfBytes;
                 const int row = c & 127;
-#pragma unroll 4
-                for (int d = 0; d < DP; d += 8) {
-                    uint32_t w[4];
-                    eight(d, w);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) w[i] = pack_f16(lo(w[i]) * up, hi(w[i]) * up);
-                    *(uint4*)(dst + (d >> 6) * kBoxBytes + row * 128 + ((((d >> 3) & 7) ^ (row & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
-                }
-                sm.temp[jobs & 1][c] = p.inv_temp * kLog2e * pow2(e - 14);
+                *(uint4*)(sQ + (c >> 7) * kHalfBytes + (d >> 6) * kBoxBytes + row * 128 + ((((d >> 3) & 7) ^ (row & 7)) << 4)) =
+                    make_uint4(pack_f16(y[0] * up, y[1] * up), pack_f16(y[2] * up, y[3] * up), pack_f16(y[4] * up, y[5] * up), pack_f16(y[6] * up, y[7] * up));
+                if (d == 0) sm.temp[jobs & 1][c] = p.inv_temp * kLog2e * pow2(e - 14);
             }
             fence_async_smem();
             mbar_arrive(&sm.bars[Q_FULL0 + (jobs & 1)]);
 
             for (int pos = first; pos < j.end; ++pos, ++step) {
-                const int key0 = kStep * (j.steps - 1 - pos), st = step & 1, slot = step % kScaleSlots;
-                if (key0 + kStep > least) {  // keys that some queries do not see: 0 * NaN would be NaN
-                    bool nan = false;
+                const int key0 = kStep * (j.steps - 1 - pos), st = values ? step & 1 : 0;
+                ok = mbar_wait(raw_full, step & 1, abort_flag) && mbar_wait(&sm.bars[values ? V_EMPTY0 + st : K_EMPTY], (ph_e >> st) & 1, abort_flag);
+                ph_e ^= 1u << st;
+                if (!ok) break;
+                uint8_t* const dst = values ? sV + st * kHalfBytes : sK;
+                const bool edge = values && key0 + kStep > least;  // keys that some queries do not see: 0 * NaN would be NaN
+                bool nan = false;
+#pragma unroll 2
+                for (int i = gw; i < kStep / kRowsALoad; i += group) {
+                    const int row = kRowsALoad * i + row0;
+                    uint4 x = *(const uint4*)(raw + row * DP + 16 * chunk);
+                    if (edge && key0 + row >= least) {
+                        uint32_t* const w[4] = {&x.x, &x.y, &x.z, &x.w};
 #pragma unroll
-                    for (int i = 0; i < kPasses; ++i) {
-                        if (key0 + row0 + dr * i < least) continue;
-                        uint32_t* const w = (uint32_t*)&vx[i];
-#pragma unroll
-                        for (int x = 0; x < 4; ++x) {
-                            const uint32_t bad = (((w[x] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7;
-                            if (bad) nan = true;
-                            w[x] &= ~(bad * 255u);
+                        for (int e = 0; e < 4; ++e) {
+                            const uint32_t bad = (((*w[e] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7;
+                            if (bad && key0 + row < j.keys) nan = true;
+                            *w[e] = key0 + row < j.keys ? *w[e] & ~(bad * 255u) : 0u;
                         }
                     }
-                    if (nan) *(volatile uint32_t*)&sm.nan_job[jobs & 1] = jobs + 1;
-                }
-                __syncwarp();
-                if (lane == 0) {
-#pragma unroll
-                    for (int g = 0; g < 2; ++g) {
-                        sm.ks[slot][2 * cw + g] = sk[g];
-                        sm.vs[slot][2 * cw + g] = sv[g];
-                    }
-                    mbar_arrive(&sm.bars[SC_FULL0 + slot]);
-                }
-                ok = mbar_wait(&sm.bars[K_EMPTY0 + st], (ph_ke >> st) & 1, abort_flag);
-                ph_ke ^= 1u << st;
-                if (!ok) break;
-#pragma unroll
-                for (int i = 0; i < kPasses; ++i) {
                     uint32_t y[8];
-                    codes_to_f16(kx[i].x, y[0], y[1]);
-                    codes_to_f16(kx[i].y, y[2], y[3]);
-                    codes_to_f16(kx[i].z, y[4], y[5]);
-                    codes_to_f16(kx[i].w, y[6], y[7]);
+                    codes_to_f16(x.x, y[0], y[1]);
+                    codes_to_f16(x.y, y[2], y[3]);
+                    codes_to_f16(x.z, y[4], y[5]);
+                    codes_to_f16(x.w, y[6], y[7]);
+                    if (values)
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            const float2 f = __half22float2(*(const __half2*)&y[e]);
+                            y[e] = pack_bf16(f.x, f.y);
+                        }
+                    // 8 values (16 bytes) of a row: [128 rows][64 values] boxes, 128-byte swizzle
                     const uint4 a = make_uint4(y[0], y[1], y[2], y[3]), b = make_uint4(y[4], y[5], y[6], y[7]);
-                    uint8_t* const dst = sK + st * kHalfBytes;
-                    *(uint4*)(dst + place(row0 + dr * i, flip)) = flip ? b : a;
-                    *(uint4*)(dst + place(row0 + dr * i, flip ^ 1)) = flip ? a : b;
+                    const int c0 = 2 * chunk + flip, c1 = c0 ^ 1;
+                    *(uint4*)(dst + (c0 >> 3) * kBoxBytes + row * 128 + (((c0 & 7) ^ (row & 7)) << 4)) = flip ? b : a;
+                    *(uint4*)(dst + (c1 >> 3) * kBoxBytes + row * 128 + (((c1 & 7) ^ (row & 7)) << 4)) = flip ? a : b;
                 }
+                if (nan) *(volatile uint32_t*)&sm.nan_job[jobs & 3] = jobs + 1;
                 fence_async_smem();
-                mbar_arrive(&sm.bars[K_FULL0 + st]);
-                ok = mbar_wait(&sm.bars[V_EMPTY0 + st], (ph_ve >> st) & 1, abort_flag);
-                ph_ve ^= 1u << st;
+                mbar_arrive(&sm.bars[values ? V_FULL0 + st : K_FULL]);
+                mbar_arrive(&sm.bars[values ? READ_V : READ_K]);
+                if (gw == 0) ok = mbar_wait(&sm.bars[values ? READ_V : READ_K], step & 1, abort_flag);  // the whole group has read the codes
                 if (!ok) break;
-#pragma unroll
-                for (int i = 0; i < kPasses; ++i) {
-                    uint32_t y[8];
-                    codes_to_f16(vx[i].x, y[0], y[1]);
-                    codes_to_f16(vx[i].y, y[2], y[3]);
-                    codes_to_f16(vx[i].z, y[4], y[5]);
-                    codes_to_f16(vx[i].w, y[6], y[7]);
-#pragma unroll
-                    for (int x = 0; x < 8; ++x) {
-                        const float2 f = __half22float2(*(const __half2*)&y[x]);
-                        y[x] = pack_bf16(f.x, f.y);
-                    }
-                    const uint4 a = make_uint4(y[0], y[1], y[2], y[3]), b = make_uint4(y[4], y[5], y[6], y[7]);
-                    uint8_t* const dst = sV + st * kHalfBytes;
-                    *(uint4*)(dst + place(row0 + dr * i, flip)) = flip ? b : a;
-                    *(uint4*)(dst + place(row0 + dr * i, flip ^ 1)) = flip ? a : b;
-                }
-                fence_async_smem();
-                mbar_arrive(&sm.bars[V_FULL0 + st]);
                 if (pos + 1 < j.end) load(pos + 1);
             }
             ++jobs;
@@ -310,13 +319,13 @@ __global__ void __launch_bounds__(kThreads, 1) cached_tc_kernel(const __grid_con
         const SmemDesc dq = make_desc(smem_u32(sQ), 0, 1024), dk = make_desc(smem_u32(sK), 0, 1024), dv = make_desc(smem_u32(sV), kBoxBytes, 1024);
         uint32_t ph_p = 0, ph_of = 3, step = 0, jobs = 0;
         bool ok = true;
-        const auto scores = [&](int t, uint32_t st) {
-            const SmemDesc a = {dq.lo + t * (kHalfBytes >> 4), dq.hi}, b = {dk.lo + st * (kHalfBytes >> 4), dk.hi};
+        const auto scores = [&](int t) {
+            const SmemDesc a = {dq.lo + t * (kHalfBytes >> 4), dq.hi};
 #pragma unroll
             for (int i = 0; i < DP / 16; ++i) {
                 const uint32_t off = (i >> 2) * kBoxBytes + (i & 3) * 32;
-                if (i == 0) mma_ss<false>(leader, tmem + kColS + 128 * t, a, off, b, off, idesc_s);
-                else mma_ss<true>(leader, tmem + kColS + 128 * t, a, off, b, off, idesc_s);
+                if (i == 0) mma_ss<false>(leader, tmem + kColS + 128 * t, a, off, dk, off, idesc_s);
+                else mma_ss<true>(leader, tmem + kColS + 128 * t, a, off, dk, off, idesc_s);
             }
             mma_commit(leader, &sm.bars[S_READY0 + t]);
         };
@@ -325,14 +334,14 @@ __global__ void __launch_bounds__(kThreads, 1) cached_tc_kernel(const __grid_con
             u += j.end - j.pos;
             const int n = j.end - k.first_pos(j), halves = j.cols > 128 ? 2 : 1;
             if (n <= 0) continue;
-            ok = mbar_wait(&sm.bars[Q_FULL0 + (jobs & 1)], (jobs >> 1) & 1, abort_flag) && mbar_wait(&sm.bars[K_FULL0 + (step & 1)], (step >> 1) & 1, abort_flag);
+            ok = mbar_wait(&sm.bars[Q_FULL0 + (jobs & 1)], (jobs >> 1) & 1, abort_flag) && mbar_wait(&sm.bars[K_FULL], step & 1, abort_flag);
             if (!ok) break;
             tc_fence_after();
-            for (int t = 0; t < halves; ++t) scores(t, step & 1);
-            mma_commit(leader, &sm.bars[K_EMPTY0 + (step & 1)]);
+            for (int t = 0; t < halves; ++t) scores(t);
+            mma_commit(leader, &sm.bars[K_EMPTY]);
             if (n == 1) mma_commit(leader, &sm.bars[Q_EMPTY]);
             for (int s = 0; s < n && ok; ++s, ++step) {
-                const uint32_t st = step & 1, next = st ^ 1;
+                const uint32_t st = step & 1;
                 ok = mbar_wait(&sm.bars[V_FULL0 + st], (step >> 1) & 1, abort_flag);
                 for (int t = 0; t < halves && ok; ++t) {
                     ok = mbar_wait(&sm.bars[P_READY0 + t], (ph_p >> t) & 1, abort_flag);
@@ -354,12 +363,12 @@ __global__ void __launch_bounds__(kThreads, 1) cached_tc_kernel(const __grid_con
                     if (s + 1 == n) {
                         mma_commit(leader, &sm.bars[O_READY0 + t]);
                     } else {
-                        if (t == 0) ok = mbar_wait(&sm.bars[K_FULL0 + next], ((step + 1) >> 1) & 1, abort_flag);
+                        if (t == 0) ok = mbar_wait(&sm.bars[K_FULL], (step + 1) & 1, abort_flag);
                         if (!ok) break;
                         tc_fence_after();
-                        scores(t, next);
+                        scores(t);
                         if (t == halves - 1) {
-                            mma_commit(leader, &sm.bars[K_EMPTY0 + next]);
+                            mma_commit(leader, &sm.bars[K_EMPTY]);
                             if (s + 2 == n) mma_commit(leader, &sm.bars[Q_EMPTY]);
                         }
                     }
@@ -383,6 +392,7 @@ __global__ void __launch_bounds__(kThreads, 1) cached_tc_kernel(const __grid_con
             const int first = k.first_pos(j), n = max(0, j.end - first);
             const bool mine = c < j.cols, live = n > 0 && 128 * half < j.cols;
             float W = 1.f;
+            bool nans = false;
             if (live) {
                 ok = mbar_wait(&sm.bars[Q_FULL0 + (jobs & 1)], (jobs >> 1) & 1, abort_flag);
                 if (!ok) break;
@@ -395,21 +405,8 @@ __global__ void __launch_bounds__(kThreads, 1) cached_tc_kernel(const __grid_con
                     if (!ok) break;
                     tc_fence_after();
                     const bool masked = key0 + kStep > least;
-                    uint32_t x[32], w[16];
-                    tmem_ld32(s_base + 96, x);
-                    tmem_wait_ld(x);
-#pragma unroll
-                    for (int ch = 3; ch >= 0; --ch) {
-                        const float k0 = sm.ks[slot][2 * ch] * temp, k1 = sm.ks[slot][2 * ch + 1] * temp;
-                        float2 pw[4][4], run[4], f[4];
-                        if (masked) sweep<true>(x, k0, k1, key0 + 32 * ch, lim, pw, run);
-                        else sweep<false>(x, k0, k1, 0, 0, pw, run);
-                        if (ch > 0) tmem_ld32(s_base + 32 * (ch - 1), x);
-                        carries(run, W, f);
-                        finish(pw, f, sm.vs[slot][2 * ch], sm.vs[slot][2 * ch + 1], w);
-                        if (ch > 0) tmem_wait_ld(x);  // the weights overwrite columns of the chunk to the left
-                        tmem_st16(s_base + kColP + 16 * ch, w);
-                    }
+                    if (masked) row_step<true>(s_base, sm.ks[slot], sm.vs[slot], temp, key0, lim, W);
+                    else row_step<false>(s_base, sm.ks[slot], sm.vs[slot], temp, 0, 0, W);
                     tmem_wait_st();
                     tc_fence_before();
                     mbar_arrive(&sm.bars[P_READY0 + half]);
@@ -419,11 +416,11 @@ __global__ void __launch_bounds__(kThreads, 1) cached_tc_kernel(const __grid_con
                 ph_o ^= 1;
                 if (!ok) break;
                 tc_fence_after();
+                nans = *(volatile uint32_t*)&sm.nan_job[jobs & 3] == jobs + 1;
             } else {
                 step += n;
             }
             const bool starts_here = j.pos == 0, whole = starts_here && j.end == j.steps;
-            const bool nans = live && *(volatile uint32_t*)&sm.nan_job[jobs & 1] == jobs + 1;
             float* const slot = pl.slots + ((size_t)self * 2 + (starts_here ? 1 : 0)) * slot_floats(kTile, DP);
             const float sum = -lg2_approx(W);
             if (mine && whole) k.template store<1>(j, c, p.head_dim, {0.f}, sum, true);  // rem alone
@@ -471,15 +468,20 @@ __global__ void __launch_bounds__(kThreads, 1) cached_tc_kernel(const __grid_con
 }
 
 template <int DP>
-constexpr size_t smem_bytes(int requests) { return 6 * 128 * DP * 2 + sizeof(Small) + sizeof(int) * ((size_t)requests + 1); }
+constexpr size_t smem_bytes(int requests) { return 5 * 128 * DP * 2 + 2 * kStep * DP + sizeof(Small) + sizeof(int) * ((size_t)requests + 1); }
 static_assert(smem_bytes<128>(SBATTN_MAX_REQUESTS) + 1024 <= 232448, "shared memory of a block");
 
 template <int DP>
 int launch(const SbCacheParams& p, cudaStream_t st) {
     const Plan pl = make_plan(p, sm_count());
+    CUtensorMap km, vm;
+    const int box = p.page_tokens < kStep ? p.page_tokens : kStep;
+    if (encode_page_map(&km, p.k_codes, DP, (int64_t)p.kv_heads * p.page_tokens, p.pages, p.k_stride, box, false) != 0 ||
+        encode_page_map(&vm, p.v_codes, DP, (int64_t)p.kv_heads * p.page_tokens, p.pages, p.v_stride, box, false) != 0)
+        return kMapEncodeFailed;
     int rc = ensure_kernel_attrs((const void*)cached_tc_kernel<DP>, (int)smem_bytes<DP>(SBATTN_MAX_REQUESTS), true);
     if (rc != 0) return rc;
-    rc = launch_kernel(cached_tc_kernel<DP>, dim3((unsigned)pl.shares), dim3(kThreads), smem_bytes<DP>(p.requests), st, p, pl);
+    rc = launch_kernel(cached_tc_kernel<DP>, dim3((unsigned)pl.shares), dim3(kThreads), smem_bytes<DP>(p.requests), st, p, pl, km, vm);
     return rc != 0 ? rc : launch_join<bf16, DP, kTile>(p, pl, st);
 }
 

@@ -331,6 +331,6 @@ int encode_tile_map(CUtensorMap* map, const void* ptr, int elem_kind /*0 bf16, 2
                     int64_t B, int64_t stride_t, int64_t stride_h, int64_t stride_b, int box_rows);
 // Pages of the 8-bit cache as [pages][rows][row bytes], page_stride bytes from page to page; a box is box_rows whole rows, swizzled as wide as
 // a row is (rows of 32 bytes are not).
-int encode_page_map(CUtensorMap* map, const void* ptr, int row, int64_t rows, int64_t pages, int64_t page_stride, int box_rows);
+int encode_page_map(CUtensorMap* map, const void* ptr, int row, int64_t rows, int64_t pages, int64_t page_stride, int box_rows, bool swizzled);
 
 }  // namespace sb

@@ -46,14 +46,14 @@ int encode_tile_map(CUtensorMap* map, const void* ptr, int elem_kind, int64_t D,
     return r == CUDA_SUCCESS ? 0 : (int)r;
 }
 
-int encode_page_map(CUtensorMap* map, const void* ptr, int row, int64_t rows, int64_t pages, int64_t page_stride, int box_rows) {
+int encode_page_map(CUtensorMap* map, const void* ptr, int row, int64_t rows, int64_t pages, int64_t page_stride, int box_rows, bool swizzled) {
     std::call_once(g_once, resolve);
     if (!g_encode) return -1;
     const cuuint64_t dims[3] = {(cuuint64_t)row, (cuuint64_t)rows, (cuuint64_t)pages};
     const cuuint64_t strides[2] = {(cuuint64_t)row, (cuuint64_t)page_stride};
     const cuuint32_t box[3] = {(cuuint32_t)row, (cuuint32_t)box_rows, 1u};
     const cuuint32_t estr[3] = {1u, 1u, 1u};
-    const CUtensorMapSwizzle sw = row == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : row == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_NONE;
+    const CUtensorMapSwizzle sw = !swizzled ? CU_TENSOR_MAP_SWIZZLE_NONE : row == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : row == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_NONE;
     const auto encode = [&]() {
         return g_encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, sw,
                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
