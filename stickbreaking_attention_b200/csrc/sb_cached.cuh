@@ -17,7 +17,7 @@ struct Job {
 
 // What the host knows of a launch besides the parameters
 struct Plan {
-    int shared;          // queries' heads per key/value head
+    int shared, shift;   // queries' heads per key/value head, and its logarithm if it is a power of two, else -1
     int quads, pairs;    // q may be read four values at a time; o written, and v read, two at a time
     int octets;          // q, o and v eight at a time
     int shares;          // of the work, at most: warps or blocks of the grid
@@ -86,7 +86,7 @@ struct Jobs {
         j.tile = (int)(job % (unsigned)tiles);
         j.end = (int)min((long long)j.steps, j.pos + (stop - u));
         j.cols = min(COLS, j.n * pl.shared - j.tile * COLS);
-        j.keys = j.len - j.n + (j.tile * COLS + j.cols - 1) / pl.shared + see;
+        j.keys = j.len - j.n + token(j.tile * COLS + j.cols - 1) + see;
         return j;
     }
     __device__ __forceinline__ void request(int r, int& first, int& n, int& len) const {
@@ -102,12 +102,13 @@ struct Jobs {
     // first step, counted from the right, that holds a key which the tile sees
     __device__ __forceinline__ int first_pos(const Job& j) const { return max(j.pos, j.steps - max(1, (j.keys + STEP - 1) / STEP)); }
     // keys that column c of the tile sees
-    __device__ __forceinline__ int sees(const Job& j, int c) const { return j.len - j.n + (j.tile * COLS + c) / pl.shared + see; }
+    __device__ __forceinline__ int sees(const Job& j, int c) const { return j.len - j.n + token(j.tile * COLS + c) + see; }
+    __device__ __forceinline__ int token(int col) const { return pl.shift >= 0 ? col >> pl.shift : col / pl.shared; }  // of a request, by column
 
     __device__ __forceinline__ int row_of(const Job& j, int c, int& head) const {
-        const int col = j.tile * COLS + c;
-        head = j.g * pl.shared + col % pl.shared;
-        return j.first + col / pl.shared;
+        const int col = j.tile * COLS + c, row = token(col);
+        head = j.g * pl.shared + col - row * pl.shared;
+        return j.first + row;
     }
     // N results of one column from d0 on, and with `writes_rem` what is left of the stick
     template <int N>
@@ -226,26 +227,31 @@ __device__ __forceinline__ void join_parts(int count, int c, int lane, F slot, f
     sum = 0.f;
 #pragma unroll
     for (int i = 0; i < N; ++i) x[i] = 0.f;
+    const auto fetch = [&](int first, float (&y)[8][N]) {  // eight parts from `first` on
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            if (first + k >= count) break;
+            const float* from = slot(first + k) + c * DP + lane * N;
+            if constexpr (N == 4) *(float4*)y[k] = *(const float4*)from;
+            else if constexpr (N == 2) *(float2*)y[k] = *(const float2*)from;
+            else y[k][0] = from[0];
+        }
+    };
     for (int base = 0; base < count; base += 32) {
+        alignas(16) float y[8][N];
         float s = base + lane < count ? slot(base + lane)[COLS * DP + c] : 0.f;
+        fetch(base, y);
 #pragma unroll
         for (int off = 1; off < 32; off <<= 1) {
-            const float y = __shfl_up_sync(0xffffffffu, s, off);
-            if (lane >= off) s += y;
+            const float z = __shfl_up_sync(0xffffffffu, s, off);
+            if (lane >= off) s += z;
         }
         float right = __shfl_up_sync(0xffffffffu, s, 1);
         if (lane == 0) right = 0.f;
         const float weight = ex2(-(sum + right));
         const int n = min(32, count - base);
         for (int a = 0; a < n; a += 8) {
-            alignas(16) float y[8][N];
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                const float* from = slot(base + min(a + k, n - 1)) + c * DP + lane * N;
-                if constexpr (N == 4) *(float4*)y[k] = *(const float4*)from;
-                else if constexpr (N == 2) *(float2*)y[k] = *(const float2*)from;
-                else y[k][0] = from[0];
-            }
+            if (a > 0) fetch(base + a, y);
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
                 const float w = __shfl_sync(0xffffffffu, weight, (a + k) & 31);
@@ -275,25 +281,30 @@ __global__ void __launch_bounds__(256) cached_join_kernel(const __grid_constant_
     j.tile = seam.z;
     k.request(j.r, j.first, j.n, j.len);
     j.cols = min(COLS, j.n * pl.shared - j.tile * COLS);
-    const int c0 = 8 * blockIdx.y, cols = j.cols - c0;  // this block's columns
-    if (cols <= 0) return;
-    const int count = seam.w - b + 2, splits = cols <= 1 ? 8 : cols <= 2 ? 4 : cols <= 4 ? 2 : 1;
-    const int c = c0 + warp / splits, part = warp % splits, a0 = count * part / splits, a1 = count * (part + 1) / splits;
+    const int count = seam.w - b + 2, splits = j.cols <= 1 ? 8 : j.cols <= 2 ? 4 : j.cols <= 4 ? 2 : 1;
+    const int part = warp % splits, a0 = count * part / splits, a1 = count * (part + 1) / splits;
     float x[N], sum = 0.f;
+    if (splits == 1) {
+        for (int c = 32 * blockIdx.y + warp; c < min(j.cols, 32 * (int)blockIdx.y + 32); c += 8) {
+            join_parts<DP, COLS>(count, c, lane, [&](int a) { return pl.slots + ((size_t)(b - 1 + a) * 2 + (a == 0 ? 1 : 0)) * slot_floats(COLS, DP); }, x, sum);
+            k.store(j, c, lane * N, x, sum, lane == 0);
+        }
+        return;
+    }
+    const int c = warp / splits;
+    if (blockIdx.y > 0) return;
     if (c < j.cols)
         join_parts<DP, COLS>(a1 - a0, c, lane, [&](int a) { return pl.slots + ((size_t)(b - 1 + a0 + a) * 2 + (a0 + a == 0 ? 1 : 0)) * slot_floats(COLS, DP); }, x, sum);
-    if (splits > 1) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) xs[warp][lane * N + i] = x[i];
-        if (lane == 0) sums[warp] = sum;
-        __syncthreads();
-        if (part != 0) return;
-        for (int s = 1; s < splits; ++s) {
-            const float weight = ex2(-sum);
+    for (int i = 0; i < N; ++i) xs[warp][lane * N + i] = x[i];
+    if (lane == 0) sums[warp] = sum;
+    __syncthreads();
+    if (part != 0) return;
+    for (int s = 1; s < splits; ++s) {
+        const float weight = ex2(-sum);
 #pragma unroll
-            for (int i = 0; i < N; ++i) x[i] = fmaf(weight, xs[warp + s][lane * N + i], x[i]);
-            sum += sums[warp + s];
-        }
+        for (int i = 0; i < N; ++i) x[i] = fmaf(weight, xs[warp + s][lane * N + i], x[i]);
+        sum += sums[warp + s];
     }
     if (c < j.cols) k.store(j, c, lane * N, x, sum, lane == 0);
 }
@@ -302,6 +313,9 @@ __global__ void __launch_bounds__(256) cached_join_kernel(const __grid_constant_
 inline Plan make_plan(const SbCacheParams& p, int shares) {
     Plan pl;
     pl.shared = p.heads / p.kv_heads;
+    pl.shift = -1;
+    for (int i = 0; i < 17; ++i)
+        if (pl.shared == 1 << i) pl.shift = i;
     const int64_t size = p.dtype == SBATTN_F32 ? 4 : 2;
     const auto even = [&](const SbMat& m, int n) { return (((uintptr_t)m.ptr | (uintptr_t)(m.stride_h * size) | (uintptr_t)(m.stride_t * size)) & (n * size - 1)) == 0; };
     pl.quads = p.head_dim % 4 == 0 && even(p.q, 4);
@@ -318,7 +332,7 @@ inline size_t plan_bytes(int64_t shares, int cols, int dp) { return align_up(16 
 template <typename T, int DP, int COLS>
 int launch_join(const SbCacheParams& p, const Plan& pl, cudaStream_t st) {
     if (pl.shares < 2) return 0;
-    return launch_kernel(cached_join_kernel<T, DP, COLS>, dim3((unsigned)pl.shares - 1, (COLS + 7) / 8), dim3(256), 0, st, p, pl);
+    return launch_kernel(cached_join_kernel<T, DP, COLS>, dim3((unsigned)pl.shares - 1, (COLS + 31) / 32), dim3(256), 0, st, p, pl);
 }
 
 }  // namespace cached

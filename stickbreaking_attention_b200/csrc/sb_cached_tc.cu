@@ -412,6 +412,12 @@ __global__ void __launch_bounds__(kThreads, 1) cached_tc_kernel(const __grid_con
                     mbar_arrive(&sm.bars[P_READY0 + half]);
                 }
                 if (!ok) break;
+                if (mine && p.v.ptr) {  // for the end of the job
+                    int h;
+                    const int t = k.row_of(j, c, h);
+                    const char* v = (const char*)p.v.ptr + 2 * (j.g * p.v.stride_h + t * p.v.stride_t);
+                    for (int b = 0; b < 2 * p.head_dim; b += 128) asm volatile("prefetch.global.L1 [%0];" ::"l"(v + b));
+                }
                 ok = mbar_wait(&sm.bars[O_READY0 + half], ph_o, abort_flag);
                 ph_o ^= 1;
                 if (!ok) break;
