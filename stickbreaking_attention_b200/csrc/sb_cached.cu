@@ -31,6 +31,7 @@ using namespace sm100;
 using namespace cached;
 
 constexpr int kCols = 8;       // queries that share a key's product
+constexpr int kJobCost = 3;    // steps that a job costs besides its own
 constexpr int kColStride = 40; // floats from column to column in the exchange buffer: 4-byte stores and 8-byte loads without bank conflicts
 
 __host__ __device__ constexpr int warps(int dp) { return dp == 128 ? 12 : 8; }
@@ -92,7 +93,7 @@ template <int DP> __device__ __forceinline__ int place_of(int key) {  // 16 * ha
 template <typename T, int DP>
 __global__ void __launch_bounds__(32 * warps(DP), blocks_per_sm(DP))
 cached_kernel(const __grid_constant__ SbCacheParams p, const __grid_constant__ Plan pl, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
-    using K = Jobs<T, DP, kCols, 32>;
+    using K = Jobs<T, DP, kCols, 32, kJobCost>;
     constexpr bool kSplitQ = sizeof(T) == 4;
     constexpr int ST = stages(DP), KW = DP / 16, VW = DP / 32, M = DP / 16, kWarps = warps(DP), kThreads = 32 * kWarps;
     extern __shared__ uint8_t raw[];
@@ -132,11 +133,11 @@ cached_kernel(const __grid_constant__ SbCacheParams p, const __grid_constant__ P
     const int box = min(32, P);
     const auto next_job = [&]() {
         const Job j = k.open(iu, w1, ir);
-        if (j.pos > 0 && lane == 0) {  // the first job of this share: the join kernel's block of this seam takes it if it started in the share before
-            const long long first = iu - j.pos, last = first + j.steps, before = units * (self - 1) / shares;
+        if (!j.starts && lane == 0) {  // the first job of this share: the join kernel's block of this seam takes it if it started in the share before
+            const long long first = iu - j.raw, last = first + j.steps + kJobCost, before = units * (self - 1) / shares;
             if (first >= before) pl.seams[self] = make_int4(j.r, j.g, j.tile, (int)((last * shares - 1) / units));  // the share of unit last - 1
         }
-        iu += j.end - j.pos;
+        iu += j.take;
         ir = j.r;
         ig = j.g;
         isteps = j.steps;
@@ -234,7 +235,7 @@ cached_kernel(const __grid_constant__ SbCacheParams p, const __grid_constant__ P
             for (int w = 0; w < KW; ++w) {
                 const int d = DP == 128 ? 16 * (cc + 4 * (w >> 2)) + 4 * (w & 3) : DP == 64 ? 16 * cc + 4 * w : 8 * cc + 4 * w;
                 nq[w] = Four{T(0.f), T(0.f), T(0.f), T(0.f)};
-                if (rr < cj.cols) {
+                if (rr < cj.cols && pos < end) {
                     if (pl.quads) {
                         if (d < p.head_dim) nq[w] = *(const Four*)(q + d);
                     } else {
@@ -464,7 +465,7 @@ cached_kernel(const __grid_constant__ SbCacheParams p, const __grid_constant__ P
         // the share's part of this job: the result, or a partial one
         working = false;
         const Job cj = ws.job[which];
-        const bool starts_here = cj.pos == 0;
+        const bool starts_here = cj.starts;
         if (packed)
 #pragma unroll
             for (int m = 0; m < M; ++m)
@@ -482,7 +483,7 @@ cached_kernel(const __grid_constant__ SbCacheParams p, const __grid_constant__ P
                 x[2 * m + 1] = acc[m][2 + c];
             }
             const float sum = ws.carry[col].x + ws.carry[col].y;
-            if (starts_here && cj.end == cj.steps) {
+            if (starts_here && cj.ends) {
                 k.store(cj, col, d0, x, sum, rr == 0);
             } else {
 #pragma unroll
@@ -513,7 +514,7 @@ cached_kernel(const __grid_constant__ SbCacheParams p, const __grid_constant__ P
 int64_t grid_of(const SbCacheParams& p) {
     const int64_t all = (int64_t)sm_count() * blocks_per_sm(p.row);
     const int64_t shared = p.heads / p.kv_heads, tiles = ((int64_t)p.tokens * shared + kCols - 1) / kCols + p.requests;
-    const int64_t steps = ((int64_t)p.width * p.page_tokens + 31) / 32, most = tiles * (steps > 0 ? steps : 1) * p.kv_heads;  // no more units than this
+    const int64_t steps = ((int64_t)p.width * p.page_tokens + 31) / 32, most = tiles * ((steps > 0 ? steps : 1) + kJobCost) * p.kv_heads;  // no more units than this
     return most < all ? (most < 1 ? 1 : most) : all;
 }
 

@@ -11,8 +11,10 @@ namespace cached {
 struct Job {
     int r, g, tile;      // request, key/value head, tile of columns
     int first, n, len;   // rows of q of the request, tokens
-    int pos, end, steps; // 32-key steps, counted from the right: [pos, end) of steps
+    int raw, take;       // first unit of this share's part of the job, and units
+    int pos, end, steps; // steps of keys, counted from the right: [pos, end) of steps
     int cols, keys;      // columns of the tile, keys that its last column sees
+    bool starts, ends;   // with its first unit in this share, with its last one
 };
 
 // What the host knows of a launch besides the parameters
@@ -44,8 +46,9 @@ __device__ __forceinline__ float rcp(float x) {
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-// The line of work: every request's tiles of COLS queries, per key/value head, in steps of STEP keys
-template <typename T, int DP, int COLS, int STEP>
+// The line of work: every request's tiles of COLS queries, per key/value head, in steps of STEP keys.  What a job costs besides its steps (its queries, its
+// results) counts as COST units ahead of them, so that shares with more jobs have fewer steps.
+template <typename T, int DP, int COLS, int STEP, int COST>
 struct Jobs {
     const SbCacheParams& p;
     const Plan& pl;
@@ -54,7 +57,7 @@ struct Jobs {
 
     static __device__ __forceinline__ long long units_of(const Plan& pl, int len, int n, int see) {  // per key/value head
         const int tiles = (n * pl.shared + COLS - 1) / COLS, keys = len - 1 + see;
-        return (long long)tiles * max(1, (keys + STEP - 1) / STEP);
+        return (long long)tiles * (max(1, (keys + STEP - 1) / STEP) + COST);
     }
     // the last request whose units start at or before u
     __device__ __forceinline__ int find(long long u) const {
@@ -74,17 +77,22 @@ struct Jobs {
         const int tiles = (j.n * pl.shared + COLS - 1) / COLS;
         j.steps = max(1, (j.len - 1 + see + STEP - 1) / STEP);
         const unsigned long long in = (unsigned long long)(u - (long long)starts[r] * p.kv_heads);
+        const unsigned cost = (unsigned)j.steps + COST;
         unsigned long long job;
         if (in >> 32) {
-            job = in / (unsigned)j.steps;
-            j.pos = (int)(in % (unsigned)j.steps);
+            job = in / cost;
+            j.raw = (int)(in % cost);
         } else {
-            job = (unsigned)in / (unsigned)j.steps;
-            j.pos = (int)((unsigned)in % (unsigned)j.steps);
+            job = (unsigned)in / cost;
+            j.raw = (int)((unsigned)in % cost);
         }
         j.g = (int)(job / (unsigned)tiles);
         j.tile = (int)(job % (unsigned)tiles);
-        j.end = (int)min((long long)j.steps, j.pos + (stop - u));
+        j.take = (int)min((long long)cost - j.raw, stop - u);
+        j.pos = max(0, j.raw - COST);
+        j.end = max(0, j.raw + j.take - COST);
+        j.starts = j.raw == 0;
+        j.ends = j.raw + j.take == (int)cost;
         j.cols = min(COLS, j.n * pl.shared - j.tile * COLS);
         j.keys = j.len - j.n + token(j.tile * COLS + j.cols - 1) + see;
         return j;
@@ -274,7 +282,7 @@ __global__ void __launch_bounds__(256) cached_join_kernel(const __grid_constant_
     const int b = blockIdx.x + 1, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int4 seam = pl.seams[b];
     if (seam.x < 0) return;
-    const Jobs<T, DP, COLS, 1> k{p, pl, nullptr, p.attend_current ? 1 : 0};
+    const Jobs<T, DP, COLS, 1, 0> k{p, pl, nullptr, p.attend_current ? 1 : 0};
     Job j;
     j.r = seam.x;
     j.g = seam.y;

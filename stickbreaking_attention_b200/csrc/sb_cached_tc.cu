@@ -27,6 +27,7 @@ using bf16 = __nv_bfloat16;
 
 constexpr int kThreads = 512, kMmaWarp = 15, kConverters = 7, kValueWarps = 4;
 constexpr int kTile = 256, kStep = 128;  // queries of a tile, keys of a step
+constexpr int kJobCost = 4;              // steps that a job costs besides its own
 constexpr uint32_t kTmemCols = 512, kColS = 0, kColO = 256, kColP = 64;
 constexpr int kScaleSlots = 4;
 enum Bar { Q_FULL0, Q_FULL1, Q_EMPTY, K_FULL, K_EMPTY, RAW_K, RAW_V, READ_K, READ_V, V_FULL0, V_FULL1, V_EMPTY0, V_EMPTY1, SC_FULL0, SC_FULL1, SC_FULL2, SC_FULL3,
@@ -128,7 +129,7 @@ __device__ __forceinline__ void row_step(uint32_t s_base, const float* ks, const
 
 template <int DP>
 __global__ void __launch_bounds__(kThreads, 1) cached_tc_kernel(const __grid_constant__ SbCacheParams p, const __grid_constant__ Plan pl, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
-    using J = Jobs<bf16, DP, kTile, kStep>;
+    using J = Jobs<bf16, DP, kTile, kStep, kJobCost>;
     constexpr int kHalfBytes = 128 * DP * 2, kBoxBytes = 128 * 128;
     extern __shared__ __align__(1024) uint8_t smem[];
     uint8_t* const sQ = smem;                       // two halves
@@ -189,7 +190,7 @@ __global__ void __launch_bounds__(kThreads, 1) cached_tc_kernel(const __grid_con
         bool ok = true;
         for (long long u = u0; u < u1 && ok;) {
             const Job j = k.open(u, u1, r0);
-            u += j.end - j.pos;
+            u += j.take;
             const int first = k.first_pos(j);
             if (first >= j.end) continue;
             const int least = k.sees(j, 0);
@@ -331,7 +332,7 @@ __global__ void __launch_bounds__(kThreads, 1) cached_tc_kernel(const __grid_con
         };
         for (long long u = u0; u < u1 && ok;) {
             const Job j = k.open(u, u1, r0);
-            u += j.end - j.pos;
+            u += j.take;
             const int n = j.end - k.first_pos(j), halves = j.cols > 128 ? 2 : 1;
             if (n <= 0) continue;
             ok = mbar_wait(&sm.bars[Q_FULL0 + (jobs & 1)], (jobs >> 1) & 1, abort_flag) && mbar_wait(&sm.bars[K_FULL], step & 1, abort_flag);
@@ -384,11 +385,11 @@ __global__ void __launch_bounds__(kThreads, 1) cached_tc_kernel(const __grid_con
         bool ok = true;
         for (long long u = u0; u < u1 && ok;) {
             const Job j = k.open(u, u1, r0);
-            if (j.pos > 0 && tid == 0) {  // the first job of this share: the join kernel's blocks of this seam take it if it started in the share before
-                const long long start = u - j.pos, last = start + j.steps, before = units * (self - 1) / shares;
+            if (!j.starts && tid == 0) {  // the first job of this share: the join kernel's blocks of this seam take it if it started in the share before
+                const long long start = u - j.raw, last = start + j.steps + kJobCost, before = units * (self - 1) / shares;
                 if (start >= before) pl.seams[self] = make_int4(j.r, j.g, j.tile, (int)((last * shares - 1) / units));
             }
-            u += j.end - j.pos;
+            u += j.take;
             const int first = k.first_pos(j), n = max(0, j.end - first);
             const bool mine = c < j.cols, live = n > 0 && 128 * half < j.cols;
             float W = 1.f;
@@ -426,7 +427,7 @@ __global__ void __launch_bounds__(kThreads, 1) cached_tc_kernel(const __grid_con
             } else {
                 step += n;
             }
-            const bool starts_here = j.pos == 0, whole = starts_here && j.end == j.steps;
+            const bool starts_here = j.starts, whole = j.starts && j.ends;
             float* const slot = pl.slots + ((size_t)self * 2 + (starts_here ? 1 : 0)) * slot_floats(kTile, DP);
             const float sum = -lg2_approx(W);
             if (mine && whole) k.template store<1>(j, c, p.head_dim, {0.f}, sum, true);  // rem alone
