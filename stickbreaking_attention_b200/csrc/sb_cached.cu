@@ -99,6 +99,7 @@ cached_kernel(const __grid_constant__ SbCacheParams p, const __grid_constant__ P
     extern __shared__ uint8_t raw[];
     uint8_t* const sm = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);
     __shared__ uint32_t gave_up;
+    __shared__ volatile long long all_units;  // here, not in registers
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rr = lane >> 2, cc = lane & 3;
     uint8_t* const ring = sm + (size_t)warp * ST * stage_bytes(DP);
     WarpScratch<ST>& ws = ((WarpScratch<ST>*)(sm + Layout<DP>::scratch))[warp];
@@ -116,15 +117,22 @@ cached_kernel(const __grid_constant__ SbCacheParams p, const __grid_constant__ P
     pdl_launch_dependents();
 
     const long long carry = scan_requests<K, kThreads>(p, pl, starts, see);
-    const long long units = carry * p.kv_heads;
     // one share of the units per warp, neighbouring ones on different SMs; no warp waits for another from here on
-    const long long shares = max(1ll, min((long long)gridDim.x * kWarps, units)), self = (long long)warp * gridDim.x + blockIdx.x;
-    const long long w1 = min(units, units * (self + 1) / shares);
+    const auto self = [&]() { return (int)(warp * gridDim.x + blockIdx.x); };
+    const auto shares_of = [&](long long units) { return (int)max(1ll, min((long long)gridDim.x * kWarps, units)); };
+    long long iu, w1;  // units of this share that are to come
+    {
+        const long long units = carry * p.kv_heads;
+        const int shares = shares_of(units);
+        if (threadIdx.x == 0) all_units = units;
+        iu = min(units, quotient(units * self(), shares));
+        w1 = min(units, quotient(units * (self() + 1), shares));
+    }
+    __syncthreads();
     const K k{p, pl, starts, see};
-    if (lane == 0) pl.seams[self] = make_int4(-1, 0, 0, 0);
+    if (lane == 0) pl.seams[2 * self()] = make_int4(-1, 0, 0, 0);
 
     // ---- loads: the next step to load is ipos of a job (of request ir, head ig); lane l holds the pages and scales of the l-th step of a batch of 32
-    long long iu = min(units, units * self / shares);
     int ir = k.find(iu), ig = 0, isteps = 0, ikeys = 0, which = 0;
     bool pending = false;  // that job has not been taken over by the steps below
     int istage = 0, ipos = 0, ibatch = 0, iend = 0, loaded = 0;
@@ -133,10 +141,7 @@ cached_kernel(const __grid_constant__ SbCacheParams p, const __grid_constant__ P
     const int box = min(32, P);
     const auto next_job = [&]() {
         const Job j = k.open(iu, w1, ir);
-        if (!j.starts && lane == 0) {  // the first job of this share: the join kernel's block of this seam takes it if it started in the share before
-            const long long first = iu - j.raw, last = first + j.steps + kJobCost, before = units * (self - 1) / shares;
-            if (first >= before) pl.seams[self] = make_int4(j.r, j.g, j.tile, (int)((last * shares - 1) / units));  // the share of unit last - 1
-        }
+        if (!j.starts && lane == 0) k.mark(j, iu, all_units, shares_of(all_units), self());
         iu += j.take;
         ir = j.r;
         ig = j.g;
@@ -146,6 +151,11 @@ cached_kernel(const __grid_constant__ SbCacheParams p, const __grid_constant__ P
         iend = j.end;
         pending = true;
         if (lane == 0) ws.job[which ^ 1] = j;
+        if (rr < j.cols && 128 * cc < p.head_dim * (int)sizeof(T)) {  // its queries, ahead of the loads of its codes
+            int h;
+            const int t = k.row_of(j, rr, h);
+            asm volatile("prefetch.global.L1 [%0];" ::"l"((const char*)p.q.ptr + sizeof(T) * (h * p.q.stride_h + t * p.q.stride_t) + 128 * cc));
+        }
     };
     const auto load_step = [&]() {
         if (ipos == ibatch) {
@@ -471,7 +481,7 @@ cached_kernel(const __grid_constant__ SbCacheParams p, const __grid_constant__ P
             for (int m = 0; m < M; ++m)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) acc[m][i] += __shfl_xor_sync(0xffffffffu, acc[m][i], 2);
-        float* const slot = pl.slots + ((size_t)self * 2 + (starts_here ? 1 : 0)) * slot_floats(kCols, DP);
+        float* const slot = pl.slots + ((size_t)self() * 2 + (starts_here ? 1 : 0)) * slot_floats(kCols, DP);
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
             const int col = 2 * cc + c, d0 = rr * 4 * VW;
@@ -503,7 +513,7 @@ cached_kernel(const __grid_constant__ SbCacheParams p, const __grid_constant__ P
             }
         }
         if (lane == 0) {
-            pl.seams[self] = make_int4(-1, 0, 0, 0);
+            pl.seams[2 * self()] = make_int4(-1, 0, 0, 0);
             atomicOr(p.status, SBATTN_ST_TIMEOUT);
         }
     }

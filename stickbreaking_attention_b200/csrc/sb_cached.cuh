@@ -24,7 +24,8 @@ struct Plan {
     int octets;          // q, o and v eight at a time
     int shares;          // of the work, at most: warps or blocks of the grid
     float* slots;        // [shares][2] partial results: of a job that goes on from the share before, and of one that starts here and goes on
-    int4* seams;         // [shares]: (request or -1, head, tile, last share) of the job that a share's first unit goes on with, if it started in the share before
+    int4* seams;         // [shares][2]: of the job that a share's first unit goes on with, if it started in the share before: (first row of q or -1, rows,
+                         // head, tile), (last share, 0, 0, 0)
 };
 
 // floats of a partial result: [column][d], then the sums
@@ -46,6 +47,11 @@ __device__ __forceinline__ float rcp(float x) {
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// a / b of non-negative numbers, in 32 bits where they fit
+__device__ __forceinline__ long long quotient(long long a, long long b) {
+    return (a | b) >> 32 ? a / b : (long long)((unsigned)a / (unsigned)b);
+}
+
 // The line of work: every request's tiles of COLS queries, per key/value head, in steps of STEP keys.  What a job costs besides its steps (its queries, its
 // results) counts as COST units ahead of them, so that shares with more jobs have fewer steps.
 template <typename T, int DP, int COLS, int STEP, int COST>
@@ -58,6 +64,13 @@ struct Jobs {
     static __device__ __forceinline__ long long units_of(const Plan& pl, int len, int n, int see) {  // per key/value head
         const int tiles = (n * pl.shared + COLS - 1) / COLS, keys = len - 1 + see;
         return (long long)tiles * (max(1, (keys + STEP - 1) / STEP) + COST);
+    }
+    // the seam of the job of unit u, which is raw units into it, for the join kernel: this share's if the job started in the share before
+    __device__ __forceinline__ void mark(const Job& j, long long u, long long units, long long shares, long long self) const {
+        const long long first = u - j.raw, last = first + j.steps + COST;
+        if (first < quotient(units * (self - 1), shares)) return;
+        pl.seams[2 * self] = make_int4(j.first, j.n, j.g, j.tile);
+        pl.seams[2 * self + 1] = make_int4((int)quotient(last * shares - 1, units), 0, 0, 0);  // the share of unit last - 1
     }
     // the last request whose units start at or before u
     __device__ __forceinline__ int find(long long u) const {
@@ -280,16 +293,16 @@ __global__ void __launch_bounds__(256) cached_join_kernel(const __grid_constant_
     pdl_wait();
     pdl_launch_dependents();
     const int b = blockIdx.x + 1, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int4 seam = pl.seams[b];
+    const int4 seam = pl.seams[2 * b], seam1 = pl.seams[2 * b + 1];
     if (seam.x < 0) return;
     const Jobs<T, DP, COLS, 1, 0> k{p, pl, nullptr, p.attend_current ? 1 : 0};
     Job j;
-    j.r = seam.x;
-    j.g = seam.y;
-    j.tile = seam.z;
-    k.request(j.r, j.first, j.n, j.len);
+    j.first = seam.x;
+    j.n = seam.y;
+    j.g = seam.z;
+    j.tile = seam.w;
     j.cols = min(COLS, j.n * pl.shared - j.tile * COLS);
-    const int count = seam.w - b + 2, splits = j.cols <= 1 ? 8 : j.cols <= 2 ? 4 : j.cols <= 4 ? 2 : 1;
+    const int count = seam1.x - b + 2, splits = j.cols <= 1 ? 8 : j.cols <= 2 ? 4 : j.cols <= 4 ? 2 : 1;
     const int part = warp % splits, a0 = count * part / splits, a1 = count * (part + 1) / splits;
     float x[N], sum = 0.f;
     if (splits == 1) {
@@ -332,10 +345,10 @@ inline Plan make_plan(const SbCacheParams& p, int shares) {
     pl.shares = shares;
     char* w = (char*)p.workspace;
     pl.seams = (int4*)w;
-    pl.slots = (float*)(w + align_up(16 * (size_t)shares, 256));
+    pl.slots = (float*)(w + align_up(32 * (size_t)shares, 256));
     return pl;
 }
-inline size_t plan_bytes(int64_t shares, int cols, int dp) { return align_up(16 * (size_t)shares, 256) + (size_t)shares * 2 * slot_floats(cols, dp) * sizeof(float); }
+inline size_t plan_bytes(int64_t shares, int cols, int dp) { return align_up(32 * (size_t)shares, 256) + (size_t)shares * 2 * slot_floats(cols, dp) * sizeof(float); }
 
 template <typename T, int DP, int COLS>
 int launch_join(const SbCacheParams& p, const Plan& pl, cudaStream_t st) {

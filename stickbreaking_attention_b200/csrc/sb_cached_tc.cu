@@ -168,10 +168,10 @@ __global__ void __launch_bounds__(kThreads, 1) cached_tc_kernel(const __grid_con
     const long long carry = scan_requests<J, kThreads>(p, pl, starts, see);
     const long long units = *abort_flag ? 0 : carry * p.kv_heads;
     const long long shares = max(1ll, min((long long)gridDim.x, units)), self = blockIdx.x;
-    const long long u0 = min(units, units * self / shares), u1 = min(units, units * (self + 1) / shares);
+    const long long u0 = min(units, quotient(units * self, shares)), u1 = min(units, quotient(units * (self + 1), shares));
     const J k{p, pl, starts, see};
     const int r0 = k.find(u0);
-    if (tid == 0) pl.seams[self] = make_int4(-1, 0, 0, 0);
+    if (tid == 0) pl.seams[2 * self] = make_int4(-1, 0, 0, 0);
 
     if (warp >= 8 && warp < kMmaWarp) {
         // ------------------------------------------------------------------ codes and queries to operands
@@ -385,10 +385,7 @@ __global__ void __launch_bounds__(kThreads, 1) cached_tc_kernel(const __grid_con
         bool ok = true;
         for (long long u = u0; u < u1 && ok;) {
             const Job j = k.open(u, u1, r0);
-            if (!j.starts && tid == 0) {  // the first job of this share: the join kernel's blocks of this seam take it if it started in the share before
-                const long long start = u - j.raw, last = start + j.steps + kJobCost, before = units * (self - 1) / shares;
-                if (start >= before) pl.seams[self] = make_int4(j.r, j.g, j.tile, (int)((last * shares - 1) / units));
-            }
+            if (!j.starts && tid == 0) k.mark(j, u, units, shares, self);
             u += j.take;
             const int first = k.first_pos(j), n = max(0, j.end - first);
             const bool mine = c < j.cols, live = n > 0 && 128 * half < j.cols;
@@ -469,7 +466,7 @@ __global__ void __launch_bounds__(kThreads, 1) cached_tc_kernel(const __grid_con
             if (n > 0) ++jobs;
         }
     }
-    if (*abort_flag && tid == 0) pl.seams[self] = make_int4(-1, 0, 0, 0);
+    if (*abort_flag && tid == 0) pl.seams[2 * self] = make_int4(-1, 0, 0, 0);
     tc_teardown(abort_flag, p.status, tmem, kTmemCols, kMmaWarp);
     clear_rem<bf16>(p, kThreads);
 }
