@@ -409,8 +409,18 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> cache_blocks(const Tensor& le
     c10::cuda::OptionalCUDAGuard guard(lengths.device());
     const Tensor len = lengths.contiguous(), more = new_tokens.contiguous();
     const int64_t n_pieces = sbattn_cache_pieces(R, tokens, page_tokens);
-    const auto ints = [&](at::IntArrayRef s) { return empty_like_dtype(len, s, at::kInt); };
-    const Tensor pieces = ints({n_pieces, 4}), after = ints({R}), count = ints({1}), ends = ints({R}), slots = ints({tokens});
+    // one allocation for the five results (five cost 3 us of a call of 9)
+    const Tensor all = empty_like_dtype(len, {4 * n_pieces + 2 * R + tokens + 1}, at::kInt);
+    int64_t at = 0;
+    const auto part = [&](int64_t rows, int64_t row) {
+        Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(all.storage()), all.key_set(), all.dtype());
+        t.unsafeGetTensorImpl()->set_storage_offset(all.storage_offset() + at);
+        if (row > 1) t.unsafeGetTensorImpl()->set_sizes_contiguous({rows, row});
+        else t.unsafeGetTensorImpl()->set_sizes_contiguous({rows});
+        at += rows * row;
+        return t;
+    };
+    const Tensor pieces = part(n_pieces, 4), after = part(R, 1), ends = part(R, 1), slots = part(tokens, 1), count = part(1, 1);
     SbBlocksParams p{};
     p.requests = (int32_t)R;
     p.width = (int32_t)tables.size(1);

@@ -16,11 +16,12 @@ and at the end of the step::
 Everything stays on the GPU: no call waits for it, and a step can be captured into a CUDA graph.  No counterpart in the reference, which has no
 serving path."""
 import math
-from typing import NamedTuple
+from typing import NamedTuple, Optional, Tuple
 
 import torch
 
 from .. import _lib
+from ..ops import OP_NAMESPACE, _empty_like_rows, _unit_inner
 
 
 class SbCache(NamedTuple):
@@ -40,6 +41,43 @@ class SbBlocks(NamedTuple):
     ends: torch.Tensor        # [requests] cumulative ends of the new tokens, packed one request behind the other
     slots: torch.Tensor       # [tokens] page * page_tokens + place of every new token, -1 behind the last one
     pieces: torch.Tensor      # [n, 4] (page, first new token, tokens there before, new tokens) of every page that is written, page -1 behind the last
+
+
+# ---------------------------------------------------------------------------------------------- registered operators
+# What a program that torch.compile traces calls in place of the binding: "cache_blocks", "cache_append", "attn_cached", beside the operators of
+# ops.py.  They write tables and caches in place, as the functions do.
+T = torch.Tensor
+
+
+@torch.library.custom_op(f"{OP_NAMESPACE}::cache_blocks", mutates_args={"tables", "free_pages"}, device_types="cuda")
+def _blocks_op(lengths: T, new_tokens: T, tables: T, free_pages: T, free_count: T, page_tokens: int, tokens: int) -> Tuple[T, T, T, T, T]:
+    # an operator's results may not share their memory
+    return tuple(x.clone() for x in _lib.binding().cache_blocks(lengths, new_tokens, tables, free_pages, free_count, page_tokens, tokens))
+
+
+@_blocks_op.register_fake
+def _(lengths, new_tokens, tables, free_pages, free_count, page_tokens, tokens):
+    requests = lengths.size(0)
+    m = min(requests, tokens)
+    pieces = m + min(m, tokens - m) + max(0, tokens - 2 * m) // page_tokens  # sbattn_cache_pieces
+    return tuple(lengths.new_empty(shape) for shape in ((requests,), (1,), (requests,), (tokens,), (pieces, 4)))
+
+
+@torch.library.custom_op(f"{OP_NAMESPACE}::cache_append", mutates_args={"k_codes", "v_codes", "k_scale", "v_scale"}, device_types="cuda")
+def _append_op(k: T, v: T, k_codes: T, v_codes: T, k_scale: T, v_scale: T, pieces: T) -> None:
+    _lib.binding().cache_append(k, v, k_codes, v_codes, k_scale, v_scale, pieces)
+
+
+@torch.library.custom_op(f"{OP_NAMESPACE}::attn_cached", mutates_args=(), device_types="cuda")
+def _attend_op(q: T, k_codes: T, v_codes: T, k_scale: T, v_scale: T, tables: T, lengths: T, ends: Optional[T], inv_temp: float, attend_current: bool,
+               v: Optional[T]) -> Tuple[T, T]:
+    return _lib.binding().attend_cached(q, k_codes, v_codes, k_scale, v_scale, tables, lengths, ends, inv_temp, attend_current, v)
+
+
+@_attend_op.register_fake
+def _(q, k_codes, v_codes, k_scale, v_scale, tables, lengths, ends, inv_temp, attend_current, v):
+    q = _unit_inner(q)
+    return _empty_like_rows(q), torch.empty(q.shape[:-1], dtype=q.dtype, device=q.device)
 
 
 def sb_cache(pages, heads, head_dim, page_tokens=64, device="cuda"):
@@ -68,6 +106,8 @@ def sb_cache_blocks(lengths, new_tokens, tables, free_pages, free_count, page_to
 
     Refused steps change nothing, have no new tokens and are reported by check_status(): more pages wanted than there are, a length
     outside [0, width * page_tokens], more new tokens than ``tokens``."""
+    if torch.compiler.is_compiling():
+        return SbBlocks(*_blocks_op(lengths, new_tokens, tables, free_pages, free_count, int(page_tokens), int(tokens)))
     return SbBlocks(*_lib.binding().cache_blocks(lengths, new_tokens, tables, free_pages, free_count, int(page_tokens), int(tokens)))
 
 
@@ -75,7 +115,7 @@ def sb_cache_append(k, v, cache, pieces):
     """New keys and values k, v ([heads, tokens, head_dim]; bfloat16, float16 or float32) into the cache, in place.  The scale of a page and
     head is the smallest power of two that keeps its largest finite value within 448; it grows when a larger value comes, and the codes of the tokens that are
     there are rounded to the new one.  Infinities and NaN are stored as NaN."""
-    _lib.binding().cache_append(k, v, *cache, pieces)
+    (_append_op if torch.compiler.is_compiling() else _lib.binding().cache_append)(k, v, *cache, pieces)
 
 
 def sb_attn_cached(q, cache, tables, lengths, ends=None, inv_temp=None, attend_current=False, v=None):
@@ -90,4 +130,5 @@ def sb_attn_cached(q, cache, tables, lengths, ends=None, inv_temp=None, attend_c
     as it was allocated.  No gradients."""
     if inv_temp is None:
         inv_temp = 1 / math.sqrt(q.size(-1))
-    return _lib.binding().attend_cached(q, *cache, tables, lengths, ends, float(inv_temp), bool(attend_current), v)
+    attend = _attend_op if torch.compiler.is_compiling() else _lib.binding().attend_cached
+    return attend(q, *cache, tables, lengths, ends, float(inv_temp), bool(attend_current), v)

@@ -696,3 +696,48 @@ def test_results_do_not_depend_on_the_neighbours_values():
         a.cache.v.view(torch.uint8)[page] = 127
     o2, rem2 = a.run()
     assert torch.equal(o[:, 1:], o2[:, 1:]) and torch.equal(rem[:, 1:], rem2[:, 1:])
+
+
+def test_torch_compile():
+    """A step inside torch.compile(fullgraph=True): the same bits, tables and cache included."""
+    from stickbreaking_attention_b200 import sb_attn_cached, sb_cache, sb_cache_append, sb_cache_blocks
+
+    def step(q, k, v, cache, lengths, new, tables, free, count):
+        s = sb_cache_blocks(lengths, new, tables, free, count, 16, 9)
+        sb_cache_append(k, v, cache, s.pieces)
+        o, rem = sb_attn_cached(q, cache, tables, s.lengths, s.ends, v=v)
+        return o * 2, rem, s.lengths, s.free_count, s.slots
+
+    outs = []
+    for run in (step, torch.compile(step, backend="aot_eager", fullgraph=True)):
+        g = torch.Generator(device="cuda").manual_seed(1)
+        cache, tables = sb_cache(12, 2, 64, 16), torch.full((3, 4), -1, dtype=torch.int32, device="cuda")
+        lengths, free, count = ints([0, 0, 0]), ints(np.arange(12)), ints([12])
+        for new in ([4, 0, 5], [1, 7, 1]):
+            q, k, v = (torch.randn(9, h, 64, generator=g, device="cuda").bfloat16().transpose(0, 1) for h in (4, 2, 2))
+            res = run(q, k, v, cache, lengths, ints(new), tables, free, count)
+            lengths, count = res[2], res[3]
+            outs.append((*(x.clone() for x in res), cache.k.view(torch.uint8).clone(), cache.v_scale.clone(), tables.clone(), free.clone()))
+    for a, b in zip(outs[:2], outs[2:]):
+        assert a[0].stride() == b[0].stride()
+        assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+def test_two_captured_graphs_and_an_eager_call(monkeypatch):
+    """Graphs captured one after the other (their workspaces may come from one pool) and replayed in turn, with eager calls between."""
+    monkeypatch.setenv("SBATTN_CHECK_STATUS", "0")
+    ps = [Problem([300, 77], [1, 1], heads=4, kv=2, dim=128, page=64, dtype="bf16", lean=3.0, seed=1), Problem([900, 200], [70, 65], heads=4, kv=2, dim=64, page=16, dtype="bf16", lean=3.0, seed=2)]
+    from stickbreaking_attention_b200 import sb_attn_cached
+    args = [(p.q, p.cache, ints(p.tables), ints(p.lengths), ints(np.cumsum(p.new))) for p in ps]
+    want = [p.run() for p in ps]
+    pool, graphs, outs = torch.cuda.graph_pool_handle(), [], []
+    for a in args:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, pool=pool):
+            outs.append([sb_attn_cached(*a) for _ in range(2)][1])
+        graphs.append(g)
+    for i in (0, 1, 1, 0, 1):
+        graphs[i].replay()
+        eager = ps[1 - i].run()
+        assert torch.equal(outs[i][0], want[i][0]) and torch.equal(outs[i][1], want[i][1])
+        assert torch.equal(eager[0], want[1 - i][0]) and torch.equal(eager[1], want[1 - i][1])
