@@ -551,10 +551,18 @@ int launch_row(const SbCacheParams& p, cudaStream_t st) {
 
 }  // namespace
 
-// Many queries per key: the kernel of sb_cached_tc.cu
+// Whether the kernel of sb_cached_tc.cu takes the call: bfloat16, and enough queries per key on average over the requests.  Both ways, us a call, bfloat16, by
+// queries (heads of a group times new tokens) of a request and key/value head:
+//   16 requests of 2000 tokens, 8 heads, head dim 128      8: 34 / 59   16: 51 / 62   32: 86 / 66   64: 153 / 68   256: 537 / 102   1024: 2055 / 269
+//   64 requests of 1000 tokens, 8 heads, head dim 128      8: 55 / 133  16: 89 / 136  32: 155 / 141  64: 284 / 139  256: 1024 / 194
+//   1 request of 16 000 tokens, 8 heads, head dim 128      8: 42 / 35   16: 42 / 38   32: 53 / 44   64: 82 / 45    256: 269 / 59
+// It starts more slowly, which decides where there is little work (the lengths are not known here, the room in the tables is):
+//   1 request of 2000 tokens, 8 heads, head dim 128        32: 27 / 31  64: 28 / 32   128: 33 / 35  256: 50 / 44
+//   1 request of 300 tokens, 4 heads, head dim 64          64: 13 / 19  128: 13 / 20  256: 15 / 24
 static bool many_queries(const SbCacheParams& p) {
-    const int64_t shared = p.heads / p.kv_heads;
-    return p.dtype == SBATTN_BF16 && p.row >= 64 && p.ends && p.requests > 0 && (int64_t)p.tokens * shared >= 64 * (int64_t)p.requests;
+    const int64_t columns = (int64_t)p.tokens * (p.heads / p.kv_heads);
+    return p.dtype == SBATTN_BF16 && p.row >= 64 && p.ends && p.requests > 0 && columns >= 24 * (int64_t)p.requests &&
+           (double)columns * p.kv_heads * p.width * p.page_tokens >= 2097152.;
 }
 
 size_t cached_workspace(const SbCacheParams& p) {

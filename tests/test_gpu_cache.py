@@ -279,6 +279,12 @@ class Problem:
         self.q = torch.tensor(rng.normal(0, 1, (heads, T, dim)) + tilt, device="cuda").to(DTYPES[dtype])
         self.own_v = torch.tensor(rng.normal(0, 1, (kv, T, dim)), device="cuda").to(DTYPES[dtype])
 
+    def widen(self):
+        """Room for more pages in the tables, until the work that they allow is that of the kernel for many queries."""
+        need = -(-2 ** 21 // (self.q.shape[0] * self.q.shape[1] * self.page))
+        self.tables = np.pad(self.tables, ((0, 0), (0, max(0, need - self.tables.shape[1]))), constant_values=-1)
+        return self
+
     def run(self, ends=True, **kw):
         from stickbreaking_attention_b200 import sb_attn_cached
         return sb_attn_cached(self.q, self.cache, ints(self.tables).reshape(len(self.lengths), -1), ints(self.lengths), ints(np.cumsum(self.new)) if ends else None, **kw)
@@ -342,31 +348,50 @@ def test_shared_heads(shared, dim):
 def test_several_new_tokens(dtype, shared, current, dim):
     lengths, new = [40, 1, 9, 100, 33, 300, 64, 5], [3, 1, 9, 17, 0, 70, 64, 2]
     p = Problem(lengths, new, heads=2 * shared, kv=2, dim=dim, page=16, dtype=dtype, lean=2.0, seed=1, extra_rows=5)
-    wide = dtype == "bf16" and shared == 3  # enough queries for the kernel that takes 256 at a time
-    p.check(attend_current=current, wide=wide)
-    p.check(attend_current=current, v=p.own_v, wide=wide)
+    p.check(attend_current=current)
+    p.check(attend_current=current, v=p.own_v)
 
 
 @pytest.mark.parametrize("dim, page", [(128, 64), (64, 16), (100, 32), (48, 128), (128, 16), (64, 64)])
-@pytest.mark.parametrize("shared, lengths, new", [(1, [200], [100]), (4, [70, 1000, 300], [70, 100, 41]), (1, [700, 64, 129], [300, 64, 128]), (8, [333], [33]), (3, [2500], [90])])
+@pytest.mark.parametrize("shared, lengths, new", [(1, [200], [100]), (4, [70, 1000, 300], [70, 100, 41]), (1, [700, 64, 129], [300, 64, 128]), (8, [333], [33]), (3, [2500], [90]), (1, [300, 150], [1, 60])])
 @pytest.mark.parametrize("current", [False, True])
 def test_many_queries(dim, page, shared, lengths, new, current):
     """Tiles of 256 queries, full and not, one half of them empty, sequences of one step and of many, cut into shares."""
-    p = Problem(lengths, new, heads=2 * shared, kv=2, dim=dim, page=page, dtype="bf16", lean=3.0, seed=dim + shared, extra_rows=3)
+    p = Problem(lengths, new, heads=2 * shared, kv=2, dim=dim, page=page, dtype="bf16", lean=3.0, seed=dim + shared, extra_rows=3).widen()
     p.check(attend_current=current, v=p.own_v, wide=True)
     p.check(attend_current=current, wide=True)
+
+
+def test_which_kernel_runs():
+    """Few queries per key and little work take the one kernel, many queries of bfloat16 the other."""
+    from torch.profiler import ProfilerActivity, profile
+
+    def kernels(p):
+        p.run()
+        with profile(activities=[ProfilerActivity.CUDA]) as prof:
+            p.run()
+            torch.cuda.synchronize()
+        return " ".join(e.key for e in prof.key_averages())
+    make = lambda dtype, new: Problem([300], [new], heads=8, kv=2, dim=64, page=16, dtype=dtype)  # noqa: E731
+    names = kernels(make("bf16", 60))
+    if "cached" not in names:
+        pytest.skip("the profiler records no kernels here")
+    assert "cached_tc_kernel" not in names
+    assert "cached_tc_kernel" in kernels(make("bf16", 60).widen())
+    assert "cached_tc_kernel" not in kernels(make("f16", 60).widen())
+    assert "cached_tc_kernel" not in kernels(make("bf16", 5).widen())
 
 
 def test_many_queries_many_requests():
     rng = np.random.default_rng(1)
     lengths = [int(x) for x in rng.integers(0, 400, 90)]
     new = [min(t, int(n)) for t, n in zip(lengths, rng.integers(0, 260, 90))]
-    Problem(lengths, new, heads=2, kv=1, dim=64, page=32, dtype="bf16", lean=2.0).check(wide=True)
+    Problem(lengths, new, heads=2, kv=1, dim=64, page=32, dtype="bf16", lean=2.0).widen().check(wide=True)
 
 
 @pytest.mark.parametrize("case", ["far", "strong", "hot", "scaled"])
 def test_many_queries_extreme_logits(case):
-    p = Problem([300, 150], [100, 90], heads=2, dim=64, page=16, dtype="bf16", lean=0.0, seed=3)
+    p = Problem([300, 150], [100, 90], heads=2, dim=64, page=16, dtype="bf16", lean=0.0, seed=3).widen()
     if case == "far":
         p.q = torch.full_like(p.q, -1.0)
         for r, t in enumerate(p.lengths):
@@ -378,7 +403,7 @@ def test_many_queries_extreme_logits(case):
 
 
 def test_many_queries_strides():
-    p = Problem([170, 133], [100, 60], heads=4, kv=2, dim=128, page=32, dtype="bf16", halves=True, lean=1.0)
+    p = Problem([170, 133], [100, 60], heads=4, kv=2, dim=128, page=32, dtype="bf16", halves=True, lean=1.0).widen()
     flat = p.run(v=p.own_v)
     p.q = p.q.permute(1, 0, 2).contiguous().permute(1, 0, 2)
     major = p.check(v=p.own_v.permute(1, 0, 2).contiguous().permute(1, 0, 2), wide=True)
@@ -391,7 +416,7 @@ def test_many_queries_strides():
 
 def test_many_queries_nan():
     """NaN in a value that some queries of a tile see; in a key; in a value that all see."""
-    p = Problem([350, 200], [100, 70], heads=2, dim=64, page=16, dtype="bf16", lean=1.0)
+    p = Problem([350, 200], [100, 70], heads=2, dim=64, page=16, dtype="bf16", lean=1.0).widen()
     clean_o, clean_rem = p.run()
     for key in (300, 20):  # rows 0 ... 99 are the tokens 250 ... 349
         page, place, sees = p.tables[0, key // 16], key % 16, max(0, key + 1 - 250)
@@ -415,7 +440,7 @@ def test_many_queries_nan():
 def test_many_queries_bad_pages(page_index, monkeypatch):
     from stickbreaking_attention_b200 import check_status
     monkeypatch.setenv("SBATTN_CHECK_STATUS", "0")
-    p = Problem([350, 200], [100, 70], heads=2, dim=64, page=16, dtype="bf16")
+    p = Problem([350, 200], [100, 70], heads=2, dim=64, page=16, dtype="bf16").widen()
     good = p.run()
     p.tables[0, 3] = page_index
     o, rem = p.run()
@@ -726,7 +751,7 @@ def test_torch_compile():
 def test_two_captured_graphs_and_an_eager_call(monkeypatch):
     """Graphs captured one after the other (their workspaces may come from one pool) and replayed in turn, with eager calls between."""
     monkeypatch.setenv("SBATTN_CHECK_STATUS", "0")
-    ps = [Problem([300, 77], [1, 1], heads=4, kv=2, dim=128, page=64, dtype="bf16", lean=3.0, seed=1), Problem([900, 200], [70, 65], heads=4, kv=2, dim=64, page=16, dtype="bf16", lean=3.0, seed=2)]
+    ps = [Problem([300, 77], [1, 1], heads=4, kv=2, dim=128, page=64, dtype="bf16", lean=3.0, seed=1), Problem([900, 200], [70, 65], heads=4, kv=2, dim=64, page=16, dtype="bf16", lean=3.0, seed=2).widen()]
     from stickbreaking_attention_b200 import sb_attn_cached
     args = [(p.q, p.cache, ints(p.tables), ints(p.lengths), ints(np.cumsum(p.new))) for p in ps]
     want = [p.run() for p in ps]
