@@ -230,37 +230,46 @@ __global__ void __launch_bounds__(kThreads, 1) cached_tc_kernel(const __grid_con
             ph_qe ^= 1;
             if (!ok) break;
             constexpr int kLanes = DP / 8, kRows = 32 / kLanes;  // lanes of a row, rows of a load
-#pragma unroll 6
-            for (int c = (warp - 8) * kRows + lane / kLanes; c < kTile; c += kConverters * kRows) {
-                const int d = 8 * (lane % kLanes);
-                int h = 0, t = 0;
-                if (c < j.cols) t = k.row_of(j, c, h);
-                const bf16* q = (const bf16*)p.q.ptr + h * p.q.stride_h + t * p.q.stride_t + d;
-                alignas(16) uint32_t w[4] = {0u, 0u, 0u, 0u};
-                if (c < j.cols) {
-                    if (pl.octets) {
-                        if (d < p.head_dim) *(uint4*)w = *(const uint4*)q;
-                    } else {
+            constexpr int kAhead = 7;  // loads that travel together
+            const int d = 8 * (lane % kLanes);
+#pragma unroll 1
+            for (int base = (warp - 8) * kRows + lane / kLanes; base < kTile; base += kAhead * kConverters * kRows) {
+                uint4 w[kAhead];
 #pragma unroll
-                        for (int i = 0; i < 8; ++i)
-                            if (d + i < p.head_dim) w[i >> 1] |= (uint32_t)__bfloat16_as_ushort(q[i]) << (16 * (i & 1));
+                for (int n = 0; n < kAhead; ++n) {
+                    const int c = base + n * kConverters * kRows;
+                    w[n] = make_uint4(0u, 0u, 0u, 0u);
+                    if (c >= j.cols || d >= p.head_dim) continue;
+                    int h;
+                    const int t = k.row_of(j, c, h);
+                    const bf16* q = (const bf16*)p.q.ptr + h * p.q.stride_h + t * p.q.stride_t + d;
+                    if (pl.octets) {
+                        w[n] = *(const uint4*)q;
+                    } else {
+                        const auto at = [&](int i) { return d + i < p.head_dim ? (uint32_t)__bfloat16_as_ushort(q[i]) : 0u; };
+                        w[n] = make_uint4(at(0) | at(1) << 16, at(2) | at(3) << 16, at(4) | at(5) << 16, at(6) | at(7) << 16);
                     }
                 }
-                float y[8], top = 0.f;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    y[i] = __uint_as_float(i & 1 ? w[i >> 1] & 0xffff0000u : w[i >> 1] << 16);
-                    const float a = fabsf(y[i]);
-                    if (a <= 3.4028234664e38f) top = fmaxf(top, a);
+                for (int n = 0; n < kAhead; ++n) {
+                    const int c = base + n * kConverters * kRows, row = c & 127;
+                    if (c >= kTile) break;
+                    const uint32_t x[4] = {w[n].x, w[n].y, w[n].z, w[n].w};
+                    float y[8], top = 0.f;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        y[i] = __uint_as_float(i & 1 ? x[i >> 1] & 0xffff0000u : x[i >> 1] << 16);
+                        const float a = fabsf(y[i]);
+                        if (a <= 3.4028234664e38f) top = fmaxf(top, a);
+                    }
+#pragma unroll
+                    for (int off = 1; off < kLanes; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+                    const int e = top > 0.f ? max((int)(__float_as_uint(top) >> 23) - 127, -112) : 14;  // up to 2^(e + 1)
+                    const float up = pow2(14 - e);
+                    *(uint4*)(sQ + (c >> 7) * kHalfBytes + (d >> 6) * kBoxBytes + row * 128 + ((((d >> 3) & 7) ^ (row & 7)) << 4)) =
+                        make_uint4(pack_f16(y[0] * up, y[1] * up), pack_f16(y[2] * up, y[3] * up), pack_f16(y[4] * up, y[5] * up), pack_f16(y[6] * up, y[7] * up));
+                    if (d == 0) sm.temp[jobs & 1][c] = p.inv_temp * kLog2e * pow2(e - 14);
                 }
-#pragma unroll
-                for (int off = 1; off < kLanes; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-                const int e = top > 0.f ? max((int)(__float_as_uint(top) >> 23) - 127, -112) : 14;  // up to 2^(e + 1)
-                const float up = pow2(14 - e);
-                const int row = c & 127;
-                *(uint4*)(sQ + (c >> 7) * kHalfBytes + (d >> 6) * kBoxBytes + row * 128 + ((((d >> 3) & 7) ^ (row & 7)) << 4)) =
-                    make_uint4(pack_f16(y[0] * up, y[1] * up), pack_f16(y[2] * up, y[3] * up), pack_f16(y[4] * up, y[5] * up), pack_f16(y[6] * up, y[7] * up));
-                if (d == 0) sm.temp[jobs & 1][c] = p.inv_temp * kLog2e * pow2(e - 14);
             }
             fence_async_smem();
             mbar_arrive(&sm.bars[Q_FULL0 + (jobs & 1)]);
