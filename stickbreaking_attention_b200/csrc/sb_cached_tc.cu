@@ -27,7 +27,7 @@ using bf16 = __nv_bfloat16;
 
 constexpr int kThreads = 512, kMmaWarp = 15, kConverters = 7, kValueWarps = 4;
 constexpr int kTile = 256, kStep = 128;  // queries of a tile, keys of a step
-constexpr int kJobCost = 4;              // steps that a job costs besides its own
+constexpr int kJobCost = 2;              // steps that a job costs besides its own
 constexpr uint32_t kTmemCols = 512, kColS = 0, kColO = 256, kColP = 64;
 constexpr int kScaleSlots = 4;
 enum Bar { Q_FULL0, Q_FULL1, Q_EMPTY, K_FULL, K_EMPTY, RAW_K, RAW_V, READ_K, READ_V, V_FULL0, V_FULL1, V_EMPTY0, V_EMPTY1, SC_FULL0, SC_FULL1, SC_FULL2, SC_FULL3,
