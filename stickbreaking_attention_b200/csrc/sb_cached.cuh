@@ -262,25 +262,26 @@ __device__ __forceinline__ void join_parts(int count, int c, int lane, F slot, f
         alignas(16) float y[8][N];
         float s = base + lane < count ? slot(base + lane)[COLS * DP + c] : 0.f;
         fetch(base, y);
-#pragma unroll
-        for (int off = 1; off < 32; off <<= 1) {
+        const int n = min(32, count - base);
+#pragma unroll 1
+        for (int off = 1; off < n; off <<= 1) {
             const float z = __shfl_up_sync(0xffffffffu, s, off);
             if (lane >= off) s += z;
         }
         float right = __shfl_up_sync(0xffffffffu, s, 1);
         if (lane == 0) right = 0.f;
         const float weight = ex2(-(sum + right));
-        const int n = min(32, count - base);
         for (int a = 0; a < n; a += 8) {
             if (a > 0) fetch(base + a, y);
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
-                const float w = __shfl_sync(0xffffffffu, weight, (a + k) & 31);
+                if (a + k >= n) break;
+                const float w = __shfl_sync(0xffffffffu, weight, a + k);
 #pragma unroll
-                for (int i = 0; i < N; ++i) x[i] = a + k < n ? fmaf(w, y[k][i], x[i]) : x[i];
+                for (int i = 0; i < N; ++i) x[i] = fmaf(w, y[k][i], x[i]);
             }
         }
-        sum += __shfl_sync(0xffffffffu, s, 31);
+        sum += __shfl_sync(0xffffffffu, s, n - 1);
     }
 }
 
