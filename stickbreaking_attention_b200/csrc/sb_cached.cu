@@ -17,6 +17,11 @@
 //   * the weights of 32 keys, with the scale of the values' page, are scaled by a power of two to at most 2^15 per column and split into two float16 terms
 //     (22 bits: what is lost is below float32's own rounding of the sums), the two products are added to float32 accumulators.
 // float32 queries are two float16 terms, too; 16-bit ones are scaled by a power of two per row and exact.
+//
+// Measured (a copy's bandwidth is 6 551 GB/s): 32 requests of 1000 ... 12 000 tokens, 32 heads, head dim 128, 1.32 GB of codes 228-240 us, 5 500-5 800 GB/s; one request
+// of 65 536 tokens, 8 heads 40 us, of which the steps take 18 (a bandwidth of 7 300 GB/s; what the loads cannot use is the start, lengths, tables, queries, and the
+// joins); 64 requests of 100 ... 4000 tokens, 8 heads of four queries each 46 us, 2 900 GB/s: four times the weights per key, and the steps' latency with three
+// warps a scheduler. Twelve warps with two stages each against eight with three: 239 / 284 us on the first (fewer spills, less to hide a step's latency with).
 #include "sb_cached.cuh"
 #include "sb_sm100.cuh"
 
@@ -31,7 +36,8 @@ using namespace sm100;
 using namespace cached;
 
 constexpr int kCols = 8;       // queries that share a key's product
-constexpr int kJobCost = 3;    // steps that a job costs besides its own
+constexpr int kJobCost = 3;    // steps that a job costs besides its own (64 requests, 512 jobs: 61 us with 0, 53 with 1, 49 with 2, 47 with 4; 16 requests of
+                               // a few new tokens: 29.3, 27.4, 27.3, 29.7)
 constexpr int kColStride = 40; // floats from column to column in the exchange buffer: 4-byte stores and 8-byte loads without bank conflicts
 
 __host__ __device__ constexpr int warps(int dp) { return dp == 128 ? 12 : 8; }
@@ -117,7 +123,7 @@ cached_kernel(const __grid_constant__ SbCacheParams p, const __grid_constant__ P
     pdl_launch_dependents();
 
     const long long carry = scan_requests<K, kThreads>(p, pl, starts, see);
-    // one share of the units per warp, neighbouring ones on different SMs; no warp waits for another from here on
+    // one share of the units per warp, neighbouring ones on different SMs
     const auto self = [&]() { return (int)(warp * gridDim.x + blockIdx.x); };
     const auto shares_of = [&](long long units) { return (int)max(1ll, min((long long)gridDim.x * kWarps, units)); };
     long long iu, w1;  // units of this share that are to come
