@@ -313,6 +313,8 @@ cached_kernel(const __grid_constant__ SbCacheParams p, const __grid_constant__ P
 #pragma unroll
             for (int mt = 0; mt < 2; ++mt) {
                 float s[4] = {0.f, 0.f, 0.f, 0.f};
+                // float32: matrix instructions round their sums towards zero, so the two halves of d and the low terms are summed apart
+                float s2[kSplitQ ? 2 : 1][4] = {};
                 const int ka = 16 * mt + pk, kb = ka + 8;
                 alignas(16) uint32_t wa[KW], wb[KW];
                 if constexpr (DP == 32) {
@@ -330,9 +332,12 @@ cached_kernel(const __grid_constant__ SbCacheParams p, const __grid_constant__ P
                     uint32_t a0, a1, a2, a3;
                     codes_to_f16(wa[w], a0, a2);
                     codes_to_f16(wb[w], a1, a3);
-                    mma16816(s, a0, a1, a2, a3, qh[2 * w], qh[2 * w + 1]);
-                    if (kSplitQ) mma16816(s, a0, a1, a2, a3, ql[2 * w], ql[2 * w + 1]);
+                    mma16816(kSplitQ && 2 * w >= KW ? s2[0] : s, a0, a1, a2, a3, qh[2 * w], qh[2 * w + 1]);
+                    if constexpr (kSplitQ) mma16816(s2[1], a0, a1, a2, a3, ql[2 * w], ql[2 * w + 1]);
                 }
+                if constexpr (kSplitQ)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) s[i] = s[i] + s2[0][i] + s2[1][i];
                 if (2 * cc < cols) {
                     float* const x0 = ws.x + 2 * cc * kColStride + ka;
                     x0[0] = s[0];
@@ -530,8 +535,9 @@ cached_kernel(const __grid_constant__ SbCacheParams p, const __grid_constant__ P
 int64_t grid_of(const SbCacheParams& p) {
     const int64_t all = (int64_t)sm_count() * blocks_per_sm(p.row);
     const int64_t shared = p.heads / p.kv_heads, tiles = ((int64_t)p.tokens * shared + kCols - 1) / kCols + p.requests;
-    const int64_t steps = ((int64_t)p.width * p.page_tokens + 31) / 32, most = tiles * ((steps > 0 ? steps : 1) + kJobCost) * p.kv_heads;  // no more units than this
-    return most < all ? (most < 1 ? 1 : most) : all;
+    const int64_t steps = ((int64_t)p.width * p.page_tokens + 31) / 32;
+    const double most = (double)tiles * (double)((steps > 0 ? steps : 1) + kJobCost) * p.kv_heads;  // no more units than this
+    return most < (double)all ? (most < 1. ? 1 : (int64_t)most) : all;
 }
 
 template <typename T, int DP>

@@ -462,6 +462,42 @@ def test_many_requests():
     Problem(lengths, new, heads=1, dim=32, page=16, dtype="f32", lean=2.0).check()
 
 
+def test_most_requests():
+    """2048 requests; one more is refused."""
+    from stickbreaking_attention_b200 import sb_attn_cached
+    rng = np.random.default_rng(1)
+    lengths = [int(x) for x in rng.integers(0, 20, 2048)]
+    new = [min(t, int(n)) for t, n in zip(lengths, rng.integers(0, 3, 2048))]
+    p = Problem(lengths, new, heads=1, dim=16, page=16, dtype="f32", lean=2.0)
+    p.check()
+    with pytest.raises(ValueError, match="2048 requests"):
+        sb_attn_cached(p.q, p.cache, ints(np.zeros((2049, 1))), ints(np.zeros(2049)), ints(np.zeros(2049)))
+
+
+@pytest.mark.parametrize("wide", [False, True])
+def test_long_caches(wide):
+    """Pages behind the first 4 GB of codes and their scales: read, and written by an append."""
+    from stickbreaking_attention_b200 import SbCache, sb_cache_append
+    p = Problem([300, 200], [90, 70] if wide else [1, 3], heads=8, kv=8, dim=128, page=64, dtype="bf16", lean=3.0)
+    if wide:
+        p.widen()
+    small, base = p.cache, 70000  # 64 KB a page
+    n = small.k.shape[0]
+    big = [torch.empty(base + n, *x.shape[1:], dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn) for x in small[:2]]
+    big += [torch.empty(base + n, 8, dtype=torch.float32, device="cuda") for _ in range(2)]
+    for b, x in zip(big, small):
+        (b.view(torch.uint8) if b.dtype != torch.float32 else b)[base:] = x.view(torch.uint8) if b.dtype != torch.float32 else x
+    p.cache = SbCache(*big)
+    flat = p.tables.copy()
+    p.tables = np.where(flat >= 0, flat + base, flat)
+    p.check(wide=wide)
+    x = torch.randn(8, 5, 128, device="cuda", dtype=torch.bfloat16)
+    page = int(p.tables[0, 0])
+    sb_cache_append(x, x, p.cache, ints([(page, 0, 3, 5)]))
+    wc, ws = orc.append(x.double().cpu().numpy(), p.codes[0][flat[0, 0]][None], p.scales[0][flat[0, 0]][None], [(0, 0, 3, 5)])
+    assert np.array_equal(p.cache.k[page].view(torch.uint8).cpu().numpy(), wc[0]) and np.array_equal(p.cache.k_scale[page].cpu().numpy(), ws[0].astype(np.float32))
+
+
 def test_strides_and_halves():
     p = Problem([70, 33], [4, 1], heads=4, kv=2, dim=64, page=16, dtype="bf16", halves=True, lean=1.0)
     flat = p.run(v=p.own_v)
