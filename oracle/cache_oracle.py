@@ -100,7 +100,7 @@ def attend(q, k, v, n, inv_temp, attend_current, own_v=None, wide=False):
     """One request and head in float64: q [n, D] are the last n of the L tokens of k, v [L, D].  Returns (o, rem) and, for each, a bound on
     what float32 arithmetic may be off: products summed in any order with truncated accumulations, 2 (D + 4) 2^-24 of the sum of magnitudes, which the
     weights feel once through their own score and sum(beta) times through the others; 64 steps of 2^-24 for exponentials, logarithms
-    and the two-term weights; sums of logarithms over blocks of 32 keys.  ``wide``: the kernel for many queries, which rounds its weights to bfloat16 (2^-8), multiplies 1 - beta
+    and the two-term weights; sums of logarithms over blocks of 32 keys.  ``wide``: the kernel for many queries, which rounds its weights to that many bfloat16 terms (2^-8 each), multiplies 1 - beta
 in float32 (four roundings of 2^-23 a key) and lets no 1 - beta fall below 2^-30."""
     L, D = k.shape
     u = 2.0 ** -24
@@ -116,7 +116,7 @@ in float32 (four roundings of 2^-23 a key) and lets no 1 - beta fall below 2^-30
             a = beta * np.exp(-right)
             o[i], rem[i] = a @ v[:m], np.exp(-soft.sum())
             with np.errstate(invalid="ignore", over="ignore"):
-                off = np.minimum(1.0, np.expm1(ex * (1 + beta.sum()) + u * (64 + (m / 32 + 8) * right)) + (2.0 ** -8 * 1.01 + 8 * m * u if wide else 0))
+                off = np.minimum(1.0, np.expm1(ex * (1 + beta.sum()) + u * (64 + (m / 32 + 8) * right)) + (2.0 ** (-8 * wide) * 1.01 + 8 * m * u if wide else 0))
                 to[i] = (a * off) @ np.abs(v[:m]) + 2 * (m / 32 + 40) * u * (a @ np.abs(v[:m]))
                 tr[i] = rem[i] * min(1.0, np.expm1(ex * beta.sum() + u * (64 + (m / 32 + 8) * soft.sum())) + (8 * m * u if wide else 0))
                 if wide:

@@ -563,7 +563,7 @@ int launch_row(const SbCacheParams& p, cudaStream_t st) {
 
 }  // namespace
 
-// Whether the kernel of sb_cached_tc.cu takes the call: bfloat16, and enough queries per key on average over the requests.  Both ways, us a call, bfloat16, by
+// Whether the kernel of sb_cached_tc.cu takes the call: 16-bit types, and enough queries per key on average over the requests.  Both ways, us a call, bfloat16, by
 // queries (heads of a group times new tokens) of a request and key/value head:
 //   16 requests of 2000 tokens, 8 heads, head dim 128      8: 34 / 59   16: 51 / 62   32: 86 / 66   64: 153 / 68   256: 537 / 102   1024: 2055 / 269
 //   64 requests of 1000 tokens, 8 heads, head dim 128      8: 55 / 133  16: 89 / 136  32: 155 / 141  64: 284 / 139  256: 1024 / 194
@@ -571,9 +571,12 @@ int launch_row(const SbCacheParams& p, cudaStream_t st) {
 // It starts more slowly, which decides where there is little work (the lengths are not known here, the room in the tables is):
 //   1 request of 2000 tokens, 8 heads, head dim 128        32: 27 / 31  64: 28 / 32   128: 33 / 35  256: 50 / 44
 //   1 request of 300 tokens, 4 heads, head dim 64          64: 13 / 19  128: 13 / 20  256: 15 / 24
+// float16 turns at the same places:
+//   16 requests of 2000 tokens, 8 heads, head dim 128      16: 51 / 72   32: 84 / 75   64: 150 / 76   256: 529 / 100   1024: 2027 / 282
+//   1 request of 2000 tokens, 8 heads, head dim 128        32: 27 / 28  64: 28 / 30   128: 33 / 32  256: 50 / 38
 static bool many_queries(const SbCacheParams& p) {
     const int64_t columns = (int64_t)p.tokens * (p.heads / p.kv_heads);
-    return p.dtype == SBATTN_BF16 && p.row >= 64 && p.ends && p.requests > 0 && columns >= 24 * (int64_t)p.requests &&
+    return p.dtype != SBATTN_F32 && p.row >= 64 && p.ends && p.requests > 0 && columns >= 24 * (int64_t)p.requests &&
            (double)columns * p.kv_heads * p.width * p.page_tokens >= 2097152.;
 }
 

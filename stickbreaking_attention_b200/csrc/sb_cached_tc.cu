@@ -1,11 +1,12 @@
-// Attention over the 8-bit paged cache where many queries share the keys (a conversation's next turn, a prompt in pieces): bfloat16, rows of 64 or
-// 128 bytes.  The line of work of sb_cached.cuh in tiles of 256 queries and steps of 128 keys, one share per block; the products on tcgen05.
+// Attention over the 8-bit paged cache where many queries share the keys (a conversation's next turn, a prompt in pieces): bfloat16 and float16, rows
+// of 64 or 128 bytes.  The line of work of sb_cached.cuh in tiles of 256 queries and steps of 128 keys, one share per block; the products on tcgen05.
 //
 // A tile is two halves of 128 queries (rows of tensor memory) against the same keys, which take turns as in sb_tc_fwd_pair.cu: while the row threads of
 // one turn scores into weights, the tensor cores work for the other.  Codes become 16-bit operands once per block and step: keys float16 (exact; the queries
 // are scaled by a power of two per row to at most 2^15, exact too), values bfloat16 (exact).  The scale of the keys' page goes into the factor of a
 // score, that of the values' page into the weight before it is rounded to bfloat16: one rounding of the weights, as in the forward
-// kernels, and bfloat16's range.
+// kernels, and bfloat16's range.  For float16 one rounding to bfloat16 would be eight of its own, and float16 weights would lack the range for scales that
+// differ from page to page: two bfloat16 terms (2^-16) instead, which the tensor cores, busy a third of the time, multiply one after the other.
 //
 // With e = 2^x and d = 1 + e, 1 - beta = 1 / d.  A thread owns a query; for a group of four keys entered with W, the product of 1 - beta to its right,
 // the weight of key m is e_m (product of d to its left in the group) W / (product of d of the group): one reciprocal per four keys.
@@ -13,12 +14,17 @@
 //
 // Warps of a block (512 threads, 128 registers): 0-3 / 4-7 row warps of the first / second half, 8-11 / 12-14 convert the codes of the values / keys, which
 // TMA brings to shared memory a step ahead, all of them the queries, 15 issues tcgen05.mma.
-// Tensor memory (512 columns): scores of the halves at 0 / 128 (weights overwrite the right half of their scores), sums at 256 / 384.
+// Tensor memory (512 columns): scores of the halves at 0 / 128 (weights overwrite the right half of their scores,
+// two terms the scores of the same keys), sums at 256 / 384.
 //
 // Measured: 4 requests of 2000 ... 5000 tokens, 512 new ones each, 32 heads over 8, head dim 128: 205 us, 550 TFLOP/s (70 us at the rate of a bfloat16 GEMM), where
 // the kernel of sb_cached.cu takes 1 868. A step of both halves takes 3 000 cycles of row work alone (2 560 of the special-function unit) and about 6 000 with
 // the conversions beside it: issue slots are half busy, the tensor pipe 30 %. Codes straight from global memory to the operands, unrolled: 302 us; three warps that
 // convert keys and values, 168 registers: 386; codes by TMA and all loops rolled: 251; the rest is the queries' loads side by side, joins and shares.
+// float16, 4 requests of 4000 tokens, 512 new ones, the same heads: 265 us (bfloat16 212), in the kernel of sb_cached.cu 2 002.  Errors of 18
+// calls against float64 (2-norm, the output's own rounding is 2.1e-4): o as the plain form's; rem 2.18e-4 for its 2.13e-4 at 20 000 tokens, 2.33e-4 for 2.05e-4 at 60 000.
+#include <type_traits>
+
 #include "sb_cached.cuh"
 #include "sb_tc_common.cuh"
 
@@ -84,7 +90,9 @@ __device__ __forceinline__ void carries(const float2 (&run)[2], float& W, float2
         W = f[h].x;
     }
 }
-__device__ __forceinline__ void finish(const float2 (&p)[2][4], const float2 (&f)[2], float vs, uint32_t (&w)[8]) {
+// kTwo: into two bfloat16 terms, w the leading one
+template <bool kTwo>
+__device__ __forceinline__ void finish(const float2 (&p)[2][4], const float2 (&f)[2], float vs, uint32_t (&w)[8], uint32_t (&low)[8]) {
     const float2 v = make_float2(vs, vs);  // not into f, which may be as small as 2^-120
 #pragma unroll
     for (int h = 0; h < 2; ++h)
@@ -93,6 +101,11 @@ __device__ __forceinline__ void finish(const float2 (&p)[2][4], const float2 (&f
             const float2 a = __fmul2_rn(__fmul2_rn(p[h][m], f[h]), v), b = __fmul2_rn(__fmul2_rn(p[h][m + 1], f[h]), v);
             w[4 * h + m / 2] = pack_bf16(a.x, b.x);
             w[4 * h + 2 + m / 2] = pack_bf16(a.y, b.y);
+            if (kTwo) {
+                const auto rest = [](uint32_t t, float l, float r) { return pack_bf16(l - __uint_as_float(t << 16), r - __uint_as_float(t & 0xffff0000u)); };
+                low[4 * h + m / 2] = rest(w[4 * h + m / 2], a.x, b.x);
+                low[4 * h + 2 + m / 2] = rest(w[4 * h + 2 + m / 2], a.y, b.y);
+            }
         }
 }
 __device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
@@ -101,11 +114,15 @@ __device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8])
                  : "memory");
 }
 
+// Columns of 16 keys' weights, from the first column of the scores: the right half of them, or those of the same 16 keys' scores (two terms)
+template <bool kTwo>
+__device__ __forceinline__ constexpr int weights_at(int ch) { return kTwo ? 16 * ch : kColP + 8 * ch; }
+
 // One row of a step, 32 keys at a time from the right: the scores of the next 32 travel while the weights of these are finished.  Weights go to columns of
 // scores that have been read.  A loop, not its four rounds one behind the other: the code of all roles has to stay in the instruction cache (12 % of the kernel).
-template <bool kMasked>
+template <bool kTwo, bool kMasked>
 __device__ __forceinline__ void row_step(uint32_t s_base, const float* ks, const float* vs, float temp, int key0, int lim, float& W) {
-    uint32_t u[2][16], w[8];
+    uint32_t u[2][16], w[8], low[8];
     float2 pw[2][2][4], run[2][2], f[2][2];
     tmem_ld16(s_base + 96, u[0]);
     tmem_ld16(s_base + 112, u[1]);
@@ -121,10 +138,12 @@ __device__ __forceinline__ void row_step(uint32_t s_base, const float* ks, const
         }
         carries(run[1], W, f[1]);
         carries(run[0], W, f[0]);
-        finish(pw[1], f[1], vs[ch + 1], w);
-        tmem_st8(s_base + kColP + 8 * (ch + 1), w);
-        finish(pw[0], f[0], vs[ch], w);
-        tmem_st8(s_base + kColP + 8 * ch, w);
+        finish<kTwo>(pw[1], f[1], vs[ch + 1], w, low);
+        tmem_st8(s_base + weights_at<kTwo>(ch + 1), w);
+        if (kTwo) tmem_st8(s_base + weights_at<kTwo>(ch + 1) + 8, low);
+        finish<kTwo>(pw[0], f[0], vs[ch], w, low);
+        tmem_st8(s_base + weights_at<kTwo>(ch), w);
+        if (kTwo) tmem_st8(s_base + weights_at<kTwo>(ch) + 8, low);
         if (ch > 0) {
             tmem_wait_ld(u[0]);
             tmem_wait_ld(u[1]);
@@ -132,9 +151,10 @@ __device__ __forceinline__ void row_step(uint32_t s_base, const float* ks, const
     }
 }
 
-template <int DP>
+template <typename T, int DP>
 __global__ void __launch_bounds__(kThreads, 1) cached_tc_kernel(const __grid_constant__ SbCacheParams p, const __grid_constant__ Plan pl, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
-    using J = Jobs<bf16, DP, kTile, kStep, kJobCost>;
+    using J = Jobs<T, DP, kTile, kStep, kJobCost>;
+    constexpr bool kTwo = std::is_same<T, __half>::value;  // float16: weights in two terms
     constexpr int kHalfBytes = 128 * DP * 2, kBoxBytes = 128 * 128;
     extern __shared__ __align__(1024) uint8_t smem[];
     uint8_t* const sQ = smem;                       // two halves
@@ -247,11 +267,11 @@ __global__ void __launch_bounds__(kThreads, 1) cached_tc_kernel(const __grid_con
                     if (c >= j.cols || d >= p.head_dim) continue;
                     int h;
                     const int t = k.row_of(j, c, h);
-                    const bf16* q = (const bf16*)p.q.ptr + h * p.q.stride_h + t * p.q.stride_t + d;
+                    const T* q = (const T*)p.q.ptr + h * p.q.stride_h + t * p.q.stride_t + d;
                     if (pl.octets) {
                         w[n] = *(const uint4*)q;
                     } else {
-                        const auto at = [&](int i) { return d + i < p.head_dim ? (uint32_t)__bfloat16_as_ushort(q[i]) : 0u; };
+                        const auto at = [&](int i) { return d + i < p.head_dim ? (uint32_t)*(const uint16_t*)(q + i) : 0u; };
                         w[n] = make_uint4(at(0) | at(1) << 16, at(2) | at(3) << 16, at(4) | at(5) << 16, at(6) | at(7) << 16);
                     }
                 }
@@ -263,13 +283,14 @@ __global__ void __launch_bounds__(kThreads, 1) cached_tc_kernel(const __grid_con
                     float y[8], top = 0.f;
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
-                        y[i] = __uint_as_float(i & 1 ? x[i >> 1] & 0xffff0000u : x[i >> 1] << 16);
+                        if (kTwo) y[i] = __half2float(__ushort_as_half((unsigned short)(x[i >> 1] >> 16 * (i & 1))));
+                        else y[i] = __uint_as_float(i & 1 ? x[i >> 1] & 0xffff0000u : x[i >> 1] << 16);
                         const float a = fabsf(y[i]);
                         if (a <= 3.4028234664e38f) top = fmaxf(top, a);
                     }
 #pragma unroll
                     for (int off = 1; off < kLanes; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-                    const int e = top > 0.f ? max((int)(__float_as_uint(top) >> 23) - 127, -112) : 14;  // up to 2^(e + 1)
+                    const int e = top > 0.f ? min(max((int)(__float_as_uint(top) >> 23) - 127, -112), kTwo ? 14 : 127) : 14;  // up to 2^(e + 1); float16 is never made smaller
                     const float up = pow2(14 - e);
                     *(uint4*)(sQ + (c >> 7) * kHalfBytes + (d >> 6) * kBoxBytes + row * 128 + ((((d >> 3) & 7) ^ (row & 7)) << 4)) =
                         make_uint4(pack_f16(y[0] * up, y[1] * up), pack_f16(y[2] * up, y[3] * up), pack_f16(y[4] * up, y[5] * up), pack_f16(y[6] * up, y[7] * up));
@@ -368,11 +389,12 @@ __global__ void __launch_bounds__(kThreads, 1) cached_tc_kernel(const __grid_con
                     if (!ok) break;
                     tc_fence_after();
                     const SmemDesc b = {dv.lo + st * (kHalfBytes >> 4), dv.hi};
-                    const uint32_t d = tmem + kColO + 128 * t, a = tmem + kColS + 128 * t + kColP;
+                    const uint32_t d = tmem + kColO + 128 * t, a = tmem + kColS + 128 * t;
 #pragma unroll
                     for (int i = 0; i < kStep / 16; ++i) {
-                        if (i == 0) mma_ts_dyn(leader, d, a, b, 0, idesc_o, s > 0);
-                        else mma_ts<true>(leader, d, a + i * 8, b, i * 2048, idesc_o);
+                        if (i == 0) mma_ts_dyn(leader, d, a + weights_at<kTwo>(0), b, 0, idesc_o, s > 0);
+                        else mma_ts<true>(leader, d, a + weights_at<kTwo>(i), b, i * 2048, idesc_o);
+                        if (kTwo) mma_ts<true>(leader, d, a + weights_at<kTwo>(i) + 8, b, i * 2048, idesc_o);
                     }
                     if (t == halves - 1) mma_commit(leader, &sm.bars[V_EMPTY0 + st]);
                     if (s + 1 == n) {
@@ -417,8 +439,8 @@ __global__ void __launch_bounds__(kThreads, 1) cached_tc_kernel(const __grid_con
                     if (!ok) break;
                     tc_fence_after();
                     const bool masked = key0 + kStep > least;
-                    if (masked) row_step<true>(s_base, sm.ks[slot], sm.vs[slot], temp, key0, lim, W);
-                    else row_step<false>(s_base, sm.ks[slot], sm.vs[slot], temp, 0, 0, W);
+                    if (masked) row_step<kTwo, true>(s_base, sm.ks[slot], sm.vs[slot], temp, key0, lim, W);
+                    else row_step<kTwo, false>(s_base, sm.ks[slot], sm.vs[slot], temp, 0, 0, W);
                     tmem_wait_st();
                     tc_fence_before();
                     mbar_arrive(&sm.bars[P_READY0 + half]);
@@ -482,14 +504,14 @@ __global__ void __launch_bounds__(kThreads, 1) cached_tc_kernel(const __grid_con
     }
     if (*abort_flag && tid == 0) pl.seams[2 * self] = make_int4(-1, 0, 0, 0);
     tc_teardown(abort_flag, p.status, tmem, kTmemCols, kMmaWarp);
-    clear_rem<bf16>(p, kThreads);
+    clear_rem<T>(p, kThreads);
 }
 
 template <int DP>
 constexpr size_t smem_bytes(int requests) { return 5 * 128 * DP * 2 + 2 * kStep * DP + sizeof(Small) + sizeof(int) * ((size_t)requests + 1); }
 static_assert(smem_bytes<128>(SBATTN_MAX_REQUESTS) + 1024 <= 232448, "shared memory of a block");
 
-template <int DP>
+template <typename T, int DP>
 int launch(const SbCacheParams& p, cudaStream_t st) {
     const Plan pl = make_plan(p, sm_count());
     CUtensorMap km, vm;
@@ -497,16 +519,19 @@ int launch(const SbCacheParams& p, cudaStream_t st) {
     if (encode_page_map(&km, p.k_codes, DP, (int64_t)p.kv_heads * p.page_tokens, p.pages, p.k_stride, box, false) != 0 ||
         encode_page_map(&vm, p.v_codes, DP, (int64_t)p.kv_heads * p.page_tokens, p.pages, p.v_stride, box, false) != 0)
         return kMapEncodeFailed;
-    int rc = ensure_kernel_attrs((const void*)cached_tc_kernel<DP>, (int)smem_bytes<DP>(SBATTN_MAX_REQUESTS), true);
+    int rc = ensure_kernel_attrs((const void*)cached_tc_kernel<T, DP>, (int)smem_bytes<DP>(SBATTN_MAX_REQUESTS), true);
     if (rc != 0) return rc;
-    rc = launch_kernel(cached_tc_kernel<DP>, dim3((unsigned)pl.shares), dim3(kThreads), smem_bytes<DP>(p.requests), st, p, pl, km, vm);
-    return rc != 0 ? rc : launch_join<bf16, DP, kTile>(p, pl, st);
+    rc = launch_kernel(cached_tc_kernel<T, DP>, dim3((unsigned)pl.shares), dim3(kThreads), smem_bytes<DP>(p.requests), st, p, pl, km, vm);
+    return rc != 0 ? rc : launch_join<T, DP, kTile>(p, pl, st);
 }
 
 }  // namespace
 
 size_t cached_tc_workspace(const SbCacheParams& p) { return plan_bytes(sm_count(), kTile, p.row); }
 
-int launch_cached_tc(const SbCacheParams& p, cudaStream_t st) { return p.row == 128 ? launch<128>(p, st) : launch<64>(p, st); }
+int launch_cached_tc(const SbCacheParams& p, cudaStream_t st) {
+    if (p.dtype == SBATTN_F16) return p.row == 128 ? launch<__half, 128>(p, st) : launch<__half, 64>(p, st);
+    return p.row == 128 ? launch<bf16, 128>(p, st) : launch<bf16, 64>(p, st);
+}
 
 }  // namespace sb

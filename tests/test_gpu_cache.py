@@ -294,12 +294,13 @@ class Problem:
         inv_temp = self.dim ** -0.5 if inv_temp is None else inv_temp
         q = self.q.double().cpu().numpy()
         own = v.double().cpu().numpy() if v is not None else None
+        terms = (2 if self.q.dtype == torch.float16 else 1) if wide else 0  # of bfloat16, for the weights
         outs, at = [[], [], [], []], 0
         for r, n in enumerate(self.new):
             rows = slice(at, at + n)
             at += n
             per = [orc.attend(q[h, rows], self.k[r][h * self.kv // self.heads], self.v[r][h * self.kv // self.heads], n, inv_temp, attend_current,
-                              own[h * self.kv // self.heads, rows] if own is not None else None, wide) for h in range(self.heads)]
+                              own[h * self.kv // self.heads, rows] if own is not None else None, terms) for h in range(self.heads)]
             for out, x in zip(outs, zip(*per)):
                 out.append(np.stack(x))
         return [np.concatenate(x, 1) for x in outs]
@@ -355,15 +356,16 @@ def test_several_new_tokens(dtype, shared, current, dim):
 @pytest.mark.parametrize("dim, page", [(128, 64), (64, 16), (100, 32), (48, 128), (128, 16), (64, 64)])
 @pytest.mark.parametrize("shared, lengths, new", [(1, [200], [100]), (4, [70, 1000, 300], [70, 100, 41]), (1, [700, 64, 129], [300, 64, 128]), (8, [333], [33]), (3, [2500], [90]), (1, [300, 150], [1, 60])])
 @pytest.mark.parametrize("current", [False, True])
-def test_many_queries(dim, page, shared, lengths, new, current):
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_many_queries(dim, page, shared, lengths, new, current, dtype):
     """Tiles of 256 queries, full and not, one half of them empty, sequences of one step and of many, cut into shares."""
-    p = Problem(lengths, new, heads=2 * shared, kv=2, dim=dim, page=page, dtype="bf16", lean=3.0, seed=dim + shared, extra_rows=3).widen()
+    p = Problem(lengths, new, heads=2 * shared, kv=2, dim=dim, page=page, dtype=dtype, lean=3.0, seed=dim + shared, extra_rows=3).widen()
     p.check(attend_current=current, v=p.own_v, wide=True)
     p.check(attend_current=current, wide=True)
 
 
 def test_which_kernel_runs():
-    """Few queries per key and little work take the one kernel, many queries of bfloat16 the other."""
+    """Few queries per key and little work take the one kernel, many queries of 16 bits the other."""
     from torch.profiler import ProfilerActivity, profile
 
     def kernels(p):
@@ -378,20 +380,23 @@ def test_which_kernel_runs():
         pytest.skip("the profiler records no kernels here")
     assert "cached_tc_kernel" not in names
     assert "cached_tc_kernel" in kernels(make("bf16", 60).widen())
-    assert "cached_tc_kernel" not in kernels(make("f16", 60).widen())
+    assert "cached_tc_kernel" in kernels(make("f16", 60).widen())
+    assert "cached_tc_kernel" not in kernels(make("f32", 60).widen())
     assert "cached_tc_kernel" not in kernels(make("bf16", 5).widen())
 
 
-def test_many_queries_many_requests():
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_many_queries_many_requests(dtype):
     rng = np.random.default_rng(1)
     lengths = [int(x) for x in rng.integers(0, 400, 90)]
     new = [min(t, int(n)) for t, n in zip(lengths, rng.integers(0, 260, 90))]
-    Problem(lengths, new, heads=2, kv=1, dim=64, page=32, dtype="bf16", lean=2.0).widen().check(wide=True)
+    Problem(lengths, new, heads=2, kv=1, dim=64, page=32, dtype=dtype, lean=2.0).widen().check(wide=True)
 
 
 @pytest.mark.parametrize("case", ["far", "strong", "hot", "scaled"])
-def test_many_queries_extreme_logits(case):
-    p = Problem([300, 150], [100, 90], heads=2, dim=64, page=16, dtype="bf16", lean=0.0, seed=3).widen()
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_many_queries_extreme_logits(case, dtype):
+    p = Problem([300, 150], [100, 90], heads=2, dim=64, page=16, dtype=dtype, lean=0.0, seed=3).widen()
     if case == "far":
         p.q = torch.full_like(p.q, -1.0)
         for r, t in enumerate(p.lengths):
@@ -402,21 +407,23 @@ def test_many_queries_extreme_logits(case):
     p.check(inv_temp={"far": 1.0, "strong": 4.0, "hot": 30.0, "scaled": 0.0}[case], wide=True)
 
 
-def test_many_queries_strides():
-    p = Problem([170, 133], [100, 60], heads=4, kv=2, dim=128, page=32, dtype="bf16", halves=True, lean=1.0).widen()
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_many_queries_strides(dtype):
+    p = Problem([170, 133], [100, 60], heads=4, kv=2, dim=128, page=32, dtype=dtype, halves=True, lean=1.0).widen()
     flat = p.run(v=p.own_v)
     p.q = p.q.permute(1, 0, 2).contiguous().permute(1, 0, 2)
     major = p.check(v=p.own_v.permute(1, 0, 2).contiguous().permute(1, 0, 2), wide=True)
     assert all(torch.equal(a, b) for a, b in zip(flat, major))
-    odd = torch.zeros(4, p.q.shape[1], 131, device="cuda", dtype=torch.bfloat16)
+    odd = torch.zeros(4, p.q.shape[1], 131, device="cuda", dtype=p.q.dtype)
     odd[..., 1:129] = p.q
     p.q = odd[..., 1:129]  # rows that do not start at an aligned address
     assert all(torch.equal(a, b) for a, b in zip(flat, p.run(v=p.own_v)))
 
 
-def test_many_queries_nan():
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_many_queries_nan(dtype):
     """NaN in a value that some queries of a tile see; in a key; in a value that all see."""
-    p = Problem([350, 200], [100, 70], heads=2, dim=64, page=16, dtype="bf16", lean=1.0).widen()
+    p = Problem([350, 200], [100, 70], heads=2, dim=64, page=16, dtype=dtype, lean=1.0).widen()
     clean_o, clean_rem = p.run()
     for key in (300, 20):  # rows 0 ... 99 are the tokens 250 ... 349
         page, place, sees = p.tables[0, key // 16], key % 16, max(0, key + 1 - 250)
@@ -434,6 +441,30 @@ def test_many_queries_nan():
     bad = torch.zeros_like(o, dtype=torch.bool)
     bad[0, 51:100] = True
     assert o[bad].isnan().all() and not o[~bad].isnan().any() and rem[0, 51:100].isnan().all() and int(rem.isnan().sum()) == 49
+
+
+@pytest.mark.parametrize("what", ["largest", "smallest", "far scales", "infinite"])
+def test_many_queries_float16_range(what):
+    """Queries at both ends of float16; pages of values whose scales lie 2^60 apart; an infinite query."""
+    p = Problem([300, 150], [100, 90], heads=2, dim=64, page=16, dtype="f16", lean=1.0, seed=4).widen()
+    if what == "far scales":  # results are in float16: the small pages' share of them is lost, the large ones' must not suffer
+        for r, t in enumerate(p.lengths):
+            for b in range(0, -(-t // 16), 2):
+                p.cache.v_scale[p.tables[r, b]] *= 2.0 ** -60
+                p.v[r][:, 16 * b:16 * b + 16] *= 2.0 ** -60
+        p.check(wide=True)
+        return
+    if what == "infinite":
+        clean = p.run()
+        p.q[1, 7, 3] = torch.inf
+        o, rem = p.run()
+        rest = torch.ones_like(rem, dtype=torch.bool)
+        rest[1, 7] = False
+        assert torch.equal(o[rest], clean[0][rest]) and torch.equal(rem[rest], clean[1][rest])
+        return
+    p.q = p.q * (2.0 ** 13 if what == "largest" else 2.0 ** -22)
+    assert p.q.isfinite().all() and p.q.abs().max() > 2 ** 14 if what == "largest" else (p.q.abs() < 2.0 ** -14).all()
+    p.check(inv_temp=2.0 ** -16 if what == "largest" else 2.0 ** 19, wide=True)
 
 
 @pytest.mark.parametrize("page_index", [-1, 10 ** 6])
