@@ -490,6 +490,9 @@ void cache_into(SbCacheParams& p, const Tensor& kc, const Tensor& vc, const Tens
 }
 
 void cache_append(const Tensor& k, const Tensor& v, const Tensor& kc, const Tensor& vc, const Tensor& ks, const Tensor& vs, const Tensor& pieces) {
+    TORCH_CHECK(!(at::GradMode::is_enabled() && (k.requires_grad() || v.requires_grad())),
+                "appending to the cache has no backward: call it under torch.no_grad() or with tensors that need no gradient");
+    TORCH_CHECK_NOT_IMPLEMENTED(!k._fw_grad(0).defined() && !v._fw_grad(0).defined(), "stick-breaking attention does not implement forward mode AD");
     at::NoGradGuard no_grad;
     SbCacheParams p{};
     c10::cuda::OptionalCUDAGuard guard(k.device());

@@ -114,8 +114,13 @@ def sb_cache_blocks(lengths, new_tokens, tables, free_pages, free_count, page_to
 def sb_cache_append(k, v, cache, pieces):
     """New keys and values k, v ([heads, tokens, head_dim]; bfloat16, float16 or float32) into the cache, in place.  The scale of a page and
     head is the smallest power of two that keeps its largest finite value within 448; it grows when a larger value comes, and the codes of the tokens that are
-    there are rounded to the new one.  Infinities and NaN are stored as NaN."""
-    (_append_op if torch.compiler.is_compiling() else _lib.binding().cache_append)(k, v, *cache, pieces)
+    there are rounded to the new one.  Infinities and NaN are stored as NaN.  A page is in at most one of the pieces.  No gradients."""
+    if torch.compiler.is_compiling():
+        if torch.is_grad_enabled() and (k.requires_grad or v.requires_grad):  # as the binding; a traced call does not come there in grad mode
+            raise RuntimeError("appending to the cache has no backward: call it under torch.no_grad() or with tensors that need no gradient")
+        _append_op(k, v, *cache, pieces)
+    else:
+        _lib.binding().cache_append(k, v, *cache, pieces)
 
 
 def sb_attn_cached(q, cache, tables, lengths, ends=None, inv_temp=None, attend_current=False, v=None):

@@ -665,6 +665,11 @@ def test_refusals():
     for k, v, pc in ((p.own_v, p.own_v[:, :1], pieces), (q, q, pieces), (p.own_v, p.own_v.float(), pieces), (p.own_v, p.own_v, pieces.long()), (p.own_v, p.own_v, pieces[:, :3])):
         with pytest.raises((ValueError, TypeError)):
             sb_cache_append(k, v, c, pc)
+    for k, v in ((p.own_v.clone().requires_grad_(), p.own_v), (p.own_v, p.own_v.clone().requires_grad_())):  # the cache would lose the gradient
+        with pytest.raises(RuntimeError, match="backward"):
+            sb_cache_append(k, v, c, ints([(-1, 0, 0, 0)]))
+        with torch.no_grad():
+            sb_cache_append(k, v, c, ints([(-1, 0, 0, 0)]))
     free, count = ints([0, 1]), ints([2])
     for bad in (dict(page_tokens=20), dict(lengths=n.long()), dict(new_tokens=n[:1]), dict(tables=t[:1]), dict(tokens=-1), dict(free_count=ints([1, 2])), dict(free_pages=free.cpu()),
                 dict(tables=t[:, ::2]), dict(free_pages=ints([0, 1, 2, 3])[::2]), dict(tables=t[:1].expand(2, -1))):
@@ -778,6 +783,40 @@ def test_other_streams_and_repeats():
         assert torch.equal(o, first[0]) and torch.equal(rem, first[1])
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_many_queries_on_several_streams(dtype):
+    p = Problem([700, 77, 640], [300, 40, 70], heads=4, kv=2, dim=64, page=64, dtype=dtype, lean=5.0).widen()
+    first = p.run(v=p.own_v)
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    torch.cuda.synchronize()
+    outs = []
+    for i in range(12):
+        with torch.cuda.stream(streams[i % 3]):
+            outs.append(p.run(v=p.own_v))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for out in outs for a, b in zip(out, first))
+
+
+@pytest.mark.parametrize("wide", [False, True])
+def test_broadcast_inputs(wide):
+    """One query for all heads and one value for all tokens, as views of stride 0; one row of page indexes for all requests."""
+    from stickbreaking_attention_b200 import sb_attn_cached, sb_cache_append
+    p = Problem([170, 170], [70, 60] if wide else [2, 1], heads=4, kv=2, dim=64, page=16, dtype="bf16", lean=1.0)
+    if wide:
+        p.widen()
+    T = p.q.shape[1]
+    q, v = p.q[:1].expand(4, -1, -1), p.own_v[:, :1].expand(-1, T, -1)
+    t = ints(p.tables[:1]).expand(2, -1)
+    n, ends = ints(p.lengths), ints(np.cumsum(p.new))
+    a, b = sb_attn_cached(q, p.cache, t, n, ends, v=v), sb_attn_cached(q.contiguous(), p.cache, t.contiguous(), n, ends, v=v.contiguous())
+    assert all(torch.equal(x, y) for x, y in zip(a, b)) and a[0].is_contiguous()
+    piece = ints([(int(p.tables[0, 3]), 0, 0, min(T, 16))])
+    sb_cache_append(v, v, p.cache, piece)
+    one = [x.view(torch.uint8).clone() for x in p.cache[:2]]
+    sb_cache_append(v.contiguous(), v.contiguous(), p.cache, piece)
+    assert all(torch.equal(x, y.view(torch.uint8)) for x, y in zip(one, p.cache[:2]))
+
+
 def test_results_do_not_depend_on_the_neighbours_values():
     """The same request beside others of the same lengths but other contents gives the same bits."""
     a = Problem([300, 500], [1, 3], heads=2, dim=64, page=16, dtype="bf16", lean=3.0, seed=1)
@@ -833,3 +872,13 @@ def test_two_captured_graphs_and_an_eager_call(monkeypatch):
         eager = ps[1 - i].run()
         assert torch.equal(outs[i][0], want[i][0]) and torch.equal(outs[i][1], want[i][1])
         assert torch.equal(eager[0], want[1 - i][0]) and torch.equal(eager[1], want[1 - i][1])
+
+
+def test_torch_compile_refuses_gradients():
+    from stickbreaking_attention_b200 import sb_attn_cached, sb_cache_append
+    p = Problem([50], [1], heads=2, dim=64, page=16, dtype="bf16")
+    x, piece = p.own_v.clone().requires_grad_(), ints([(-1, 0, 0, 0)])
+    with pytest.raises(Exception, match="no backward"):
+        torch.compile(lambda x: sb_cache_append(x, x, p.cache, piece))(x)
+    with pytest.raises(Exception, match="backward"):
+        torch.compile(lambda x: sb_attn_cached(x, p.cache, ints(p.tables), ints(p.lengths))[0].float().sum())(x).backward()
