@@ -574,9 +574,12 @@ int launch_row(const SbCacheParams& p, cudaStream_t st) {
 // float16 turns at the same places:
 //   16 requests of 2000 tokens, 8 heads, head dim 128      16: 51 / 72   32: 84 / 75   64: 150 / 76   256: 529 / 100   1024: 2027 / 282
 //   1 request of 2000 tokens, 8 heads, head dim 128        32: 27 / 28  64: 28 / 30   128: 33 / 32  256: 50 / 38
+// and so do rows of 32 bytes (bfloat16):
+//   16 requests of 2000 tokens, 8 heads, head dim 32       16: 39 / 47   32: 61 / 51   64: 106 / 51   256: 375 / 64    1024: 1427 / 174
+//   64 requests of 1000 tokens, 8 heads, head dim 32       16: 64 / 88   32: 112 / 92  64: 201 / 92   256: 718 / 113
 static bool many_queries(const SbCacheParams& p) {
     const int64_t columns = (int64_t)p.tokens * (p.heads / p.kv_heads);
-    return p.dtype != SBATTN_F32 && p.row >= 64 && p.ends && p.requests > 0 && columns >= 24 * (int64_t)p.requests &&
+    return p.dtype != SBATTN_F32 && p.ends && p.requests > 0 && columns >= 24 * (int64_t)p.requests &&
            (double)columns * p.kv_heads * p.width * p.page_tokens >= 2097152.;
 }
 

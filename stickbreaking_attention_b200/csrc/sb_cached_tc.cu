@@ -1,5 +1,5 @@
-// Attention over the 8-bit paged cache where many queries share the keys (a conversation's next turn, a prompt in pieces): bfloat16 and float16, rows
-// of 64 or 128 bytes.  The line of work of sb_cached.cuh in tiles of 256 queries and steps of 128 keys, one share per block; the products on tcgen05.
+// Attention over the 8-bit paged cache where many queries share the keys (a conversation's next turn, a prompt in pieces): bfloat16 and float16.
+// The line of work of sb_cached.cuh in tiles of 256 queries and steps of 128 keys, one share per block; the products on tcgen05.
 //
 // A tile is two halves of 128 queries (rows of tensor memory) against the same keys, which take turns as in sb_tc_fwd_pair.cu: while the row threads of
 // one turn scores into weights, the tensor cores work for the other.  Codes become 16-bit operands once per block and step: keys float16 (exact; the queries
@@ -23,6 +23,7 @@
 // convert keys and values, 168 registers: 386; codes by TMA and all loops rolled: 251; the rest is the queries' loads side by side, joins and shares.
 // float16, 4 requests of 4000 tokens, 512 new ones, the same heads: 265 us (bfloat16 212), in the kernel of sb_cached.cu 2 002.  Errors of 18
 // calls against float64 (2-norm, the output's own rounding is 2.1e-4): o as the plain form's; rem 2.18e-4 for its 2.13e-4 at 20 000 tokens, 2.33e-4 for 2.05e-4 at 60 000.
+// Head dim 32, the same requests and heads, bfloat16: 168 us, in the kernel of sb_cached.cu 1 408.
 #include <type_traits>
 
 #include "sb_cached.cuh"
@@ -151,9 +152,12 @@ __device__ __forceinline__ void row_step(uint32_t s_base, const float* ks, const
     }
 }
 
-template <typename T, int DP>
+// ROW: bytes of a cached row, and columns of the results; DP: values of an operand's row.  Behind a row of 32 values the operands hold what shared memory happens to:
+// the products for scores stop before it, and the columns of the sums that it reaches are not read.
+template <typename T, int ROW>
 __global__ void __launch_bounds__(kThreads, 1) cached_tc_kernel(const __grid_constant__ SbCacheParams p, const __grid_constant__ Plan pl, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
-    using J = Jobs<T, DP, kTile, kStep, kJobCost>;
+    constexpr int DP = ROW < 64 ? 64 : ROW;
+    using J = Jobs<T, ROW, kTile, kStep, kJobCost>;
     constexpr bool kTwo = std::is_same<T, __half>::value;  // float16: weights in two terms
     constexpr int kHalfBytes = 128 * DP * 2, kBoxBytes = 128 * 128;
     extern __shared__ __align__(1024) uint8_t smem[];
@@ -161,8 +165,8 @@ __global__ void __launch_bounds__(kThreads, 1) cached_tc_kernel(const __grid_con
     uint8_t* const sK = sQ + 2 * kHalfBytes;        // one stage: it is free as soon as both halves have their scores
     uint8_t* const sV = sK + kHalfBytes;            // two stages
     uint8_t* const raw_k = sV + 2 * kHalfBytes;     // codes of a step
-    uint8_t* const raw_v = raw_k + kStep * DP;
-    Small& sm = *(Small*)(raw_v + kStep * DP);
+    uint8_t* const raw_v = raw_k + kStep * ROW;
+    Small& sm = *(Small*)(raw_v + kStep * ROW);
     int* const starts = (int*)(&sm + 1);
     volatile uint32_t* const abort_flag = &sm.abort;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, see = p.attend_current ? 1 : 0, P = p.page_tokens;
@@ -202,9 +206,9 @@ __global__ void __launch_bounds__(kThreads, 1) cached_tc_kernel(const __grid_con
         // ------------------------------------------------------------------ codes and queries to operands
         const bool values = warp < 8 + kValueWarps;
         const int group = values ? kValueWarps : kConverters - kValueWarps, gw = values ? warp - 8 : warp - 8 - kValueWarps;
-        constexpr int kPerRow = DP / 16, kRowsALoad = 32 / kPerRow;  // 16-byte pieces of a row; rows a warp takes at a time
+        constexpr int kPerRow = ROW / 16, kRowsALoad = 32 / kPerRow;  // 16-byte pieces of a row; rows a warp takes at a time
         const int chunk = lane % kPerRow, row0 = lane / kPerRow;
-        const int flip = DP == 128 ? (chunk >> 2) & 1 : 0;  // which half of 16 values is stored first: all banks once
+        const int flip = ROW == 128 ? (chunk >> 2) & 1 : 0;  // which half of 16 values is stored first: all banks once
         const CUtensorMap* const map = values ? &vmap : &kmap;
         uint64_t* const raw_full = &sm.bars[values ? RAW_V : RAW_K];
         uint8_t* const raw = values ? raw_v : raw_k;
@@ -238,10 +242,10 @@ __global__ void __launch_bounds__(kThreads, 1) cached_tc_kernel(const __grid_con
                     batch += 32 / nb;
                 }
                 const int l0 = nb * (pos - (batch - 32 / nb)), i = lane - l0, key0 = kStep * (j.steps - 1 - pos), key = key0 + box * i;
-                if (i == 0) mbar_expect_tx(raw_full, min(nb, (j.keys - key0 + box - 1) / box) * box * DP);
+                if (i == 0) mbar_expect_tx(raw_full, min(nb, (j.keys - key0 + box - 1) / box) * box * ROW);
                 __syncwarp();
                 if (i >= 0 && i < nb) {
-                    if (key < j.keys) tma_load_3d(raw + box * i * DP, map, raw_full, 0, j.g * P + key % P, page);
+                    if (key < j.keys) tma_load_3d(raw + box * i * ROW, map, raw_full, 0, j.g * P + key % P, page);
                     float* const to = (values ? sm.vs : sm.ks)[issued % kScaleSlots] + i * (box / 16);
                     for (int e = 0; e < box / 16; ++e) to[e] = scale;
                 }
@@ -311,7 +315,7 @@ __global__ void __launch_bounds__(kThreads, 1) cached_tc_kernel(const __grid_con
 #pragma unroll 2
                 for (int i = gw; i < kStep / kRowsALoad; i += group) {
                     const int row = kRowsALoad * i + row0;
-                    uint4 x = *(const uint4*)(raw + row * DP + 16 * chunk);
+                    uint4 x = *(const uint4*)(raw + row * ROW + 16 * chunk);
                     if (edge && key0 + row >= least) {
                         uint32_t* const w[4] = {&x.x, &x.y, &x.z, &x.w};
 #pragma unroll
@@ -358,7 +362,7 @@ __global__ void __launch_bounds__(kThreads, 1) cached_tc_kernel(const __grid_con
         const auto scores = [&](int t) {
             const SmemDesc a = {dq.lo + t * (kHalfBytes >> 4), dq.hi};
 #pragma unroll
-            for (int i = 0; i < DP / 16; ++i) {
+            for (int i = 0; i < ROW / 16; ++i) {
                 const uint32_t off = (i >> 2) * kBoxBytes + (i & 3) * 32;
                 if (i == 0) mma_ss<false>(leader, tmem + kColS + 128 * t, a, off, dk, off, idesc_s);
                 else mma_ss<true>(leader, tmem + kColS + 128 * t, a, off, dk, off, idesc_s);
@@ -461,12 +465,12 @@ __global__ void __launch_bounds__(kThreads, 1) cached_tc_kernel(const __grid_con
                 step += n;
             }
             const bool starts_here = j.starts, whole = j.starts && j.ends;
-            float* const slot = pl.slots + ((size_t)self * 2 + (starts_here ? 1 : 0)) * slot_floats(kTile, DP);
+            float* const slot = pl.slots + ((size_t)self * 2 + (starts_here ? 1 : 0)) * slot_floats(kTile, ROW);
             const float sum = -lg2_approx(W);
             if (mine && whole) k.template store<1>(j, c, p.head_dim, {0.f}, sum, true);  // rem alone
-            if (mine && !whole) slot[kTile * DP + c] = sum;
+            if (mine && !whole) slot[kTile * ROW + c] = sum;
 #pragma unroll 1
-            for (int d0 = 0; d0 < DP; d0 += 32) {
+            for (int d0 = 0; d0 < ROW; d0 += 32) {
                 uint32_t v[32];
                 if (live) {
                     tmem_ld32(o_base + d0, v);
@@ -475,7 +479,7 @@ __global__ void __launch_bounds__(kThreads, 1) cached_tc_kernel(const __grid_con
 #pragma unroll
                     for (int i = 0; i < 32; ++i) v[i] = 0u;
                 }
-                if (live && d0 + 32 == DP) {
+                if (live && d0 + 32 == ROW) {
                     tc_fence_before();
                     mbar_arrive(&sm.bars[O_FREE0 + half]);
                 }
@@ -486,7 +490,7 @@ __global__ void __launch_bounds__(kThreads, 1) cached_tc_kernel(const __grid_con
                     for (int key = max(k.sees(j, 0), kStep * (j.steps - j.end)); key < min(lim, kStep * (j.steps - first)); ++key) {
                         const int page = p.tables[j.r * p.table_stride + key / P];
                         if (page < 0 || page >= p.pages) continue;
-                        const uint8_t* code = (const uint8_t*)p.v_codes + page * p.v_stride + ((int64_t)j.g * P + key % P) * DP + d0;
+                        const uint8_t* code = (const uint8_t*)p.v_codes + page * p.v_stride + ((int64_t)j.g * P + key % P) * ROW + d0;
 #pragma unroll
                         for (int i = 0; i < 32; ++i)
                             if ((code[i] & 127) == 127) x[i] = __int_as_float(0x7fc00000);
@@ -496,7 +500,7 @@ __global__ void __launch_bounds__(kThreads, 1) cached_tc_kernel(const __grid_con
                     k.template store<32>(j, c, d0, x, sum, false);
                 } else {
 #pragma unroll
-                    for (int i = 0; i < 32; i += 4) *(float4*)(slot + c * DP + d0 + i) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
+                    for (int i = 0; i < 32; i += 4) *(float4*)(slot + c * ROW + d0 + i) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
                 }
             }
             if (n > 0) ++jobs;
@@ -507,31 +511,32 @@ __global__ void __launch_bounds__(kThreads, 1) cached_tc_kernel(const __grid_con
     clear_rem<T>(p, kThreads);
 }
 
-template <int DP>
-constexpr size_t smem_bytes(int requests) { return 5 * 128 * DP * 2 + 2 * kStep * DP + sizeof(Small) + sizeof(int) * ((size_t)requests + 1); }
+template <int ROW>
+constexpr size_t smem_bytes(int requests) { return 5 * 128 * (ROW < 64 ? 64 : ROW) * 2 + 2 * kStep * ROW + sizeof(Small) + sizeof(int) * ((size_t)requests + 1); }
 static_assert(smem_bytes<128>(SBATTN_MAX_REQUESTS) + 1024 <= 232448, "shared memory of a block");
 
-template <typename T, int DP>
+template <typename T, int ROW>
 int launch(const SbCacheParams& p, cudaStream_t st) {
     const Plan pl = make_plan(p, sm_count());
     CUtensorMap km, vm;
     const int box = p.page_tokens < kStep ? p.page_tokens : kStep;
-    if (encode_page_map(&km, p.k_codes, DP, (int64_t)p.kv_heads * p.page_tokens, p.pages, p.k_stride, box, false) != 0 ||
-        encode_page_map(&vm, p.v_codes, DP, (int64_t)p.kv_heads * p.page_tokens, p.pages, p.v_stride, box, false) != 0)
+    if (encode_page_map(&km, p.k_codes, ROW, (int64_t)p.kv_heads * p.page_tokens, p.pages, p.k_stride, box, false) != 0 ||
+        encode_page_map(&vm, p.v_codes, ROW, (int64_t)p.kv_heads * p.page_tokens, p.pages, p.v_stride, box, false) != 0)
         return kMapEncodeFailed;
-    int rc = ensure_kernel_attrs((const void*)cached_tc_kernel<T, DP>, (int)smem_bytes<DP>(SBATTN_MAX_REQUESTS), true);
+    int rc = ensure_kernel_attrs((const void*)cached_tc_kernel<T, ROW>, (int)smem_bytes<ROW>(SBATTN_MAX_REQUESTS), true);
     if (rc != 0) return rc;
-    rc = launch_kernel(cached_tc_kernel<T, DP>, dim3((unsigned)pl.shares), dim3(kThreads), smem_bytes<DP>(p.requests), st, p, pl, km, vm);
-    return rc != 0 ? rc : launch_join<T, DP, kTile>(p, pl, st);
+    rc = launch_kernel(cached_tc_kernel<T, ROW>, dim3((unsigned)pl.shares), dim3(kThreads), smem_bytes<ROW>(p.requests), st, p, pl, km, vm);
+    return rc != 0 ? rc : launch_join<T, ROW, kTile>(p, pl, st);
 }
 
 }  // namespace
 
 size_t cached_tc_workspace(const SbCacheParams& p) { return plan_bytes(sm_count(), kTile, p.row); }
 
-int launch_cached_tc(const SbCacheParams& p, cudaStream_t st) {
-    if (p.dtype == SBATTN_F16) return p.row == 128 ? launch<__half, 128>(p, st) : launch<__half, 64>(p, st);
-    return p.row == 128 ? launch<bf16, 128>(p, st) : launch<bf16, 64>(p, st);
+template <typename T>
+static int launch_row(const SbCacheParams& p, cudaStream_t st) {
+    return p.row == 128 ? launch<T, 128>(p, st) : p.row == 64 ? launch<T, 64>(p, st) : launch<T, 32>(p, st);
 }
+int launch_cached_tc(const SbCacheParams& p, cudaStream_t st) { return p.dtype == SBATTN_F16 ? launch_row<__half>(p, st) : launch_row<bf16>(p, st); }
 
 }  // namespace sb

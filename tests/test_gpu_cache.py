@@ -353,7 +353,7 @@ def test_several_new_tokens(dtype, shared, current, dim):
     p.check(attend_current=current, v=p.own_v)
 
 
-@pytest.mark.parametrize("dim, page", [(128, 64), (64, 16), (100, 32), (48, 128), (128, 16), (64, 64)])
+@pytest.mark.parametrize("dim, page", [(128, 64), (64, 16), (100, 32), (48, 128), (128, 16), (64, 64), (32, 64), (24, 16), (17, 128)])
 @pytest.mark.parametrize("shared, lengths, new", [(1, [200], [100]), (4, [70, 1000, 300], [70, 100, 41]), (1, [700, 64, 129], [300, 64, 128]), (8, [333], [33]), (3, [2500], [90]), (1, [300, 150], [1, 60])])
 @pytest.mark.parametrize("current", [False, True])
 @pytest.mark.parametrize("dtype", ["bf16", "f16"])
@@ -421,9 +421,10 @@ def test_many_queries_strides(dtype):
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f16"])
-def test_many_queries_nan(dtype):
+@pytest.mark.parametrize("dim", [64, 32])
+def test_many_queries_nan(dtype, dim):
     """NaN in a value that some queries of a tile see; in a key; in a value that all see."""
-    p = Problem([350, 200], [100, 70], heads=2, dim=64, page=16, dtype=dtype, lean=1.0).widen()
+    p = Problem([350, 200], [100, 70], heads=2, dim=dim, page=16, dtype=dtype, lean=1.0).widen()
     clean_o, clean_rem = p.run()
     for key in (300, 20):  # rows 0 ... 99 are the tokens 250 ... 349
         page, place, sees = p.tables[0, key // 16], key % 16, max(0, key + 1 - 250)
