@@ -17,13 +17,13 @@
 // Tensor memory (512 columns): scores of the halves at 0 / 128 (weights overwrite the right half of their scores,
 // two terms the scores of the same keys), sums at 256 / 384.
 //
-// Measured: 4 requests of 2000 ... 5000 tokens, 512 new ones each, 32 heads over 8, head dim 128: 205 us, 550 TFLOP/s (70 us at the rate of a bfloat16 GEMM), where
-// the kernel of sb_cached.cu takes 1 868. A step of both halves takes 3 000 cycles of row work alone (2 560 of the special-function unit) and about 6 000 with
-// the conversions beside it: issue slots are half busy, the tensor pipe 30 %. Codes straight from global memory to the operands, unrolled: 302 us; three warps that
+// Measured: 4 requests of 2000 ... 5000 tokens, 512 new ones each, 32 heads over 8, head dim 128: 195 us, 577 TFLOP/s (70 us at the rate of a bfloat16 GEMM), where
+// the kernel of sb_cached.cu takes 1 868. The special-function unit needs 2 560 cycles for a step of both halves, which takes about 5 500: issue slots are half busy,
+// the tensor pipe 30 %, and with a quarter of the conversions (head dim 32) a step is not much shorter. Rows wait for their own results. Codes straight from global memory to the operands, unrolled: 302 us; three warps that
 // convert keys and values, 168 registers: 386; codes by TMA and all loops rolled: 251; the rest is the queries' loads side by side, joins and shares.
-// float16, 4 requests of 4000 tokens, 512 new ones, the same heads: 265 us (bfloat16 212), in the kernel of sb_cached.cu 2 002.  Errors of 18
+// float16, 4 requests of 4000 tokens, 512 new ones, the same heads: 226 us (bfloat16 203), in the kernel of sb_cached.cu 2 002.  Errors of 18
 // calls against float64 (2-norm, the output's own rounding is 2.1e-4): o as the plain form's; rem 2.18e-4 for its 2.13e-4 at 20 000 tokens, 2.33e-4 for 2.05e-4 at 60 000.
-// Head dim 32, the same requests and heads, bfloat16: 168 us, in the kernel of sb_cached.cu 1 408.
+// Head dim 32, the same requests and heads, bfloat16: 160 us, in the kernel of sb_cached.cu 1 408.
 #include <type_traits>
 
 #include "sb_cached.cuh"
@@ -119,37 +119,39 @@ __device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8])
 template <bool kTwo>
 __device__ __forceinline__ constexpr int weights_at(int ch) { return kTwo ? 16 * ch : kColP + 8 * ch; }
 
-// One row of a step, 32 keys at a time from the right: the scores of the next 32 travel while the weights of these are finished.  Weights go to columns of
-// scores that have been read.  A loop, not its four rounds one behind the other: the code of all roles has to stay in the instruction cache (12 % of the kernel).
+// One row of a step, 16 keys at a time from the right, one such group ahead: exponentials of the next keys (special functions) stand beside the weights
+// of these (arithmetic), scores of the keys after them travel.  Weights go to columns of scores that have been read.  A loop, not its rounds one behind
+// the other: the code of all roles has to stay in the instruction cache (12 % of the kernel).  32 keys at a time, first all exponentials and then all
+// weights, with spilled registers: 205 us for 195 (the case below "Measured"), float16 266 for 226; more registers for rows by setmaxnreg did not help that form.
 template <bool kTwo, bool kMasked>
 __device__ __forceinline__ void row_step(uint32_t s_base, const float* ks, const float* vs, float temp, int key0, int lim, float& W) {
     uint32_t u[2][16], w[8], low[8];
-    float2 pw[2][2][4], run[2][2], f[2][2];
-    tmem_ld16(s_base + 96, u[0]);
-    tmem_ld16(s_base + 112, u[1]);
-    tmem_wait_ld(u[0]);
-    tmem_wait_ld(u[1]);
-#pragma unroll 1
-    for (int ch = 6; ch >= 0; ch -= 2) {
-        sweep<kMasked>(u[1], ks[ch + 1] * temp, key0 + 16 * ch + 16, lim, pw[1], run[1]);
-        sweep<kMasked>(u[0], ks[ch] * temp, key0 + 16 * ch, lim, pw[0], run[0]);
-        if (ch > 0) {
-            tmem_ld16(s_base + 16 * (ch - 2), u[0]);
-            tmem_ld16(s_base + 16 * (ch - 1), u[1]);
-        }
-        carries(run[1], W, f[1]);
-        carries(run[0], W, f[0]);
-        finish<kTwo>(pw[1], f[1], vs[ch + 1], w, low);
-        tmem_st8(s_base + weights_at<kTwo>(ch + 1), w);
-        if (kTwo) tmem_st8(s_base + weights_at<kTwo>(ch + 1) + 8, low);
-        finish<kTwo>(pw[0], f[0], vs[ch], w, low);
+    float2 pw[2][2][4], run[2][2], f[2];
+    const auto swept = [&](int b, int ch) {
+        tmem_wait_ld(u[b]);
+        sweep<kMasked>(u[b], ks[ch] * temp, key0 + 16 * ch, lim, pw[b], run[b]);
+    };
+    const auto out = [&](int b, int ch) {
+        carries(run[b], W, f);
+        finish<kTwo>(pw[b], f, vs[ch], w, low);
         tmem_st8(s_base + weights_at<kTwo>(ch), w);
         if (kTwo) tmem_st8(s_base + weights_at<kTwo>(ch) + 8, low);
-        if (ch > 0) {
-            tmem_wait_ld(u[0]);
-            tmem_wait_ld(u[1]);
-        }
+    };
+    tmem_ld16(s_base + 112, u[1]);
+    swept(1, 7);
+    tmem_ld16(s_base + 96, u[0]);
+#pragma unroll 1
+    for (int ch = 7; ch > 1; ch -= 2) {
+        swept(0, ch - 1);
+        tmem_ld16(s_base + 16 * (ch - 2), u[1]);
+        out(1, ch);
+        swept(1, ch - 2);
+        tmem_ld16(s_base + 16 * (ch - 3), u[0]);
+        out(0, ch - 1);
     }
+    swept(0, 0);
+    out(1, 1);
+    out(0, 0);
 }
 
 // ROW: bytes of a cached row, and columns of the results; DP: values of an operand's row.  Behind a row of 32 values the operands hold what shared memory happens to:
