@@ -571,7 +571,7 @@ int launch_row(const SbCacheParams& p, cudaStream_t st) {
 // It starts more slowly, which decides where there is little work (the lengths are not known here, the room in the tables is):
 //   1 request of 2000 tokens, 8 heads, head dim 128        32: 27 / 31  64: 28 / 32   128: 33 / 35  256: 50 / 44
 //   1 request of 300 tokens, 4 heads, head dim 64          64: 13 / 19  128: 13 / 20  256: 15 / 24
-// float16 turns at the same places:
+// float16 turns at the same places (the second figures here and above are from before its row steps were pipelined: 0 to 15 % less now, at few columns the same):
 //   16 requests of 2000 tokens, 8 heads, head dim 128      16: 51 / 72   32: 84 / 75   64: 150 / 76   256: 529 / 100   1024: 2027 / 282
 //   1 request of 2000 tokens, 8 heads, head dim 128        32: 27 / 28  64: 28 / 30   128: 33 / 32  256: 50 / 38
 // and so do rows of 32 bytes (bfloat16):

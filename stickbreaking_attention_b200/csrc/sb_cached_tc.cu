@@ -14,6 +14,7 @@
 //
 // Warps of a block (512 threads, 128 registers): 0-3 / 4-7 row warps of the first / second half, 8-11 / 12-14 convert the codes of the values / keys, which
 // TMA brings to shared memory a step ahead, all of them the queries, 15 issues tcgen05.mma.
+// The product with the values starts with the right 64 keys while rows work on the left ones (173 -> 163 us at head dim 64, 160 -> 152 at 32, nothing at 128).
 // Tensor memory (512 columns): scores of the halves at 0 / 128 (weights overwrite the right half of their scores,
 // two terms the scores of the same keys), sums at 256 / 384.
 //
@@ -21,9 +22,9 @@
 // the kernel of sb_cached.cu takes 1 868. The special-function unit needs 2 560 cycles for a step of both halves, which takes about 5 500: issue slots are half busy,
 // the tensor pipe 30 %, and with a quarter of the conversions (head dim 32) a step is not much shorter. Rows wait for their own results. Codes straight from global memory to the operands, unrolled: 302 us; three warps that
 // convert keys and values, 168 registers: 386; codes by TMA and all loops rolled: 251; the rest is the queries' loads side by side, joins and shares.
-// float16, 4 requests of 4000 tokens, 512 new ones, the same heads: 226 us (bfloat16 203), in the kernel of sb_cached.cu 2 002.  Errors of 18
+// float16, 4 requests of 4000 tokens, 512 new ones, the same heads: 226 us (bfloat16 205), in the kernel of sb_cached.cu 2 002.  Errors of 18
 // calls against float64 (2-norm, the output's own rounding is 2.1e-4): o as the plain form's; rem 2.18e-4 for its 2.13e-4 at 20 000 tokens, 2.33e-4 for 2.05e-4 at 60 000.
-// Head dim 32, the same requests and heads, bfloat16: 160 us, in the kernel of sb_cached.cu 1 408.
+// Head dim 32, the same requests and heads, bfloat16: 152 us, in the kernel of sb_cached.cu 1 408.
 #include <type_traits>
 
 #include "sb_cached.cuh"
@@ -43,7 +44,7 @@ constexpr int kJobCost = 2;              // steps that a job costs besides its o
 constexpr uint32_t kTmemCols = 512, kColS = 0, kColO = 256, kColP = 64;
 constexpr int kScaleSlots = 4;
 enum Bar { Q_FULL0, Q_FULL1, Q_EMPTY, K_FULL, K_EMPTY, RAW_K, RAW_V, READ_K, READ_V, V_FULL0, V_FULL1, V_EMPTY0, V_EMPTY1, SC_FULL0, SC_FULL1, SC_FULL2, SC_FULL3,
-           S_READY0, S_READY1, P_READY0, P_READY1, O_READY0, O_READY1, O_FREE0, O_FREE1, kNumBars };
+           S_READY0, S_READY1, P_READY0, P_READY1, P_HALF0, P_HALF1, O_READY0, O_READY1, O_FREE0, O_FREE1, kNumBars };
 
 struct Small {  // behind the tiles
     uint64_t bars[kNumBars];
@@ -121,10 +122,12 @@ __device__ __forceinline__ constexpr int weights_at(int ch) { return kTwo ? 16 *
 
 // One row of a step, 16 keys at a time from the right, one such group ahead: exponentials of the next keys (special functions) stand beside the weights
 // of these (arithmetic), scores of the keys after them travel.  Weights go to columns of scores that have been read.  A loop, not its rounds one behind
-// the other: the code of all roles has to stay in the instruction cache (12 % of the kernel).  32 keys at a time, first all exponentials and then all
-// weights, with spilled registers: 205 us for 195 (the case below "Measured"), float16 266 for 226; more registers for rows by setmaxnreg did not help that form.
+// the other: the code of all roles has to stay in the instruction cache (12 % of the kernel).  us for 32 keys at a time, all exponentials and then all weights,
+// with spilled registers / this: 4 requests of 4000 tokens, 512 new ones, 32 heads over 8, bfloat16, head dim 128: 213 / 205, 64: 183 / 164, 32: 169 / 152,
+// float16, 128: 266 / 226.  Jobs of few steps do not gain: 64 requests of 1000 tokens, 8 heads, head dim 128, 512 columns 277 / 276, 32 columns 131 / 131, head dim 32,
+// 64 columns 93 / 96; with masked steps in this form too (twice the code) 285, 137 and 103.  More registers for rows by setmaxnreg did not help the first form.
 template <bool kTwo, bool kMasked>
-__device__ __forceinline__ void row_step(uint32_t s_base, const float* ks, const float* vs, float temp, int key0, int lim, float& W) {
+__device__ __forceinline__ void row_step(uint32_t s_base, uint64_t* half_ready, const float* ks, const float* vs, float temp, int key0, int lim, float& W) {
     uint32_t u[2][16], w[8], low[8];
     float2 pw[2][2][4], run[2][2], f[2];
     const auto swept = [&](int b, int ch) {
@@ -137,6 +140,20 @@ __device__ __forceinline__ void row_step(uint32_t s_base, const float* ks, const
         tmem_st8(s_base + weights_at<kTwo>(ch), w);
         if (kTwo) tmem_st8(s_base + weights_at<kTwo>(ch) + 8, low);
     };
+    if (kMasked) {  // few steps of a job: short code counts for more
+#pragma unroll 1
+        for (int ch = 7; ch >= 0; --ch) {
+            tmem_ld16(s_base + 16 * ch, u[0]);
+            swept(0, ch);
+            out(0, ch);
+            if (ch == 4) {
+                tmem_wait_st();
+                tc_fence_before();
+                mbar_arrive(half_ready);
+            }
+        }
+        return;
+    }
     tmem_ld16(s_base + 112, u[1]);
     swept(1, 7);
     tmem_ld16(s_base + 96, u[0]);
@@ -148,6 +165,11 @@ __device__ __forceinline__ void row_step(uint32_t s_base, const float* ks, const
         swept(1, ch - 2);
         tmem_ld16(s_base + 16 * (ch - 3), u[0]);
         out(0, ch - 1);
+        if (ch == 5) {  // the right 64 keys' weights are there, and no score under them is still to be read
+            tmem_wait_st();
+            tc_fence_before();
+            mbar_arrive(half_ready);
+        }
     }
     swept(0, 0);
     out(1, 1);
@@ -175,7 +197,7 @@ __global__ void __launch_bounds__(kThreads, 1) cached_tc_kernel(const __grid_con
     if (tid == 0) {
         for (int i = 0; i < kNumBars; ++i) {
             const bool by_all = i == Q_FULL0 || i == Q_FULL1, by_values = i == V_FULL0 || i == V_FULL1 || i == READ_V;
-            const bool by_rows = i == P_READY0 || i == P_READY1 || i == O_FREE0 || i == O_FREE1;
+            const bool by_rows = i == P_READY0 || i == P_READY1 || i == P_HALF0 || i == P_HALF1 || i == O_FREE0 || i == O_FREE1;
             mbar_init(&sm.bars[i], by_all ? 32 * kConverters : i == K_FULL || i == READ_K ? 32 * (kConverters - kValueWarps) : by_values ? 32 * kValueWarps : by_rows ? 128 : i >= SC_FULL0 && i <= SC_FULL3 ? 2 : 1);
         }
         for (int i = 0; i < 4; ++i) sm.nan_job[i] = 0;
@@ -386,8 +408,7 @@ __global__ void __launch_bounds__(kThreads, 1) cached_tc_kernel(const __grid_con
                 const uint32_t st = step & 1;
                 ok = mbar_wait(&sm.bars[V_FULL0 + st], (step >> 1) & 1, abort_flag);
                 for (int t = 0; t < halves && ok; ++t) {
-                    ok = mbar_wait(&sm.bars[P_READY0 + t], (ph_p >> t) & 1, abort_flag);
-                    ph_p ^= 1u << t;
+                    ok = mbar_wait(&sm.bars[P_HALF0 + t], (ph_p >> t) & 1, abort_flag);
                     if (ok && s == 0) {  // the sums before must have been read
                         ok = mbar_wait(&sm.bars[O_FREE0 + t], (ph_of >> t) & 1, abort_flag);
                         ph_of ^= 1u << t;
@@ -397,11 +418,18 @@ __global__ void __launch_bounds__(kThreads, 1) cached_tc_kernel(const __grid_con
                     const SmemDesc b = {dv.lo + st * (kHalfBytes >> 4), dv.hi};
                     const uint32_t d = tmem + kColO + 128 * t, a = tmem + kColS + 128 * t;
 #pragma unroll
-                    for (int i = 0; i < kStep / 16; ++i) {
-                        if (i == 0) mma_ts_dyn(leader, d, a + weights_at<kTwo>(0), b, 0, idesc_o, s > 0);
+                    for (int i = kStep / 16 - 1; i >= 0; --i) {
+                        if (i == kStep / 32 - 1) {
+                            ok = mbar_wait(&sm.bars[P_READY0 + t], (ph_p >> t) & 1, abort_flag);
+                            ph_p ^= 1u << t;
+                            if (!ok) break;
+                            tc_fence_after();
+                        }
+                        if (i == kStep / 16 - 1) mma_ts_dyn(leader, d, a + weights_at<kTwo>(i), b, i * 2048, idesc_o, s > 0);
                         else mma_ts<true>(leader, d, a + weights_at<kTwo>(i), b, i * 2048, idesc_o);
                         if (kTwo) mma_ts<true>(leader, d, a + weights_at<kTwo>(i) + 8, b, i * 2048, idesc_o);
                     }
+                    if (!ok) break;
                     if (t == halves - 1) mma_commit(leader, &sm.bars[V_EMPTY0 + st]);
                     if (s + 1 == n) {
                         mma_commit(leader, &sm.bars[O_READY0 + t]);
@@ -445,8 +473,8 @@ __global__ void __launch_bounds__(kThreads, 1) cached_tc_kernel(const __grid_con
                     if (!ok) break;
                     tc_fence_after();
                     const bool masked = key0 + kStep > least;
-                    if (masked) row_step<kTwo, true>(s_base, sm.ks[slot], sm.vs[slot], temp, key0, lim, W);
-                    else row_step<kTwo, false>(s_base, sm.ks[slot], sm.vs[slot], temp, 0, 0, W);
+                    if (masked) row_step<kTwo, true>(s_base, &sm.bars[P_HALF0 + half], sm.ks[slot], sm.vs[slot], temp, key0, lim, W);
+                    else row_step<kTwo, false>(s_base, &sm.bars[P_HALF0 + half], sm.ks[slot], sm.vs[slot], temp, 0, 0, W);
                     tmem_wait_st();
                     tc_fence_before();
                     mbar_arrive(&sm.bars[P_READY0 + half]);
