@@ -126,3 +126,56 @@ in float32 (four roundings of 2^-23 a key) and lets no 1 - beta fall below 2^-30
             o[i] += rem[i] * own_v[i]
             to[i] += tr[i] * np.abs(own_v[i])
     return o, rem, to, tr
+
+
+def attend_rows(q, k, v, n, inv_temp, attend_current, own_v=None, wide=0):
+    """attend(), all rows at once: for tests with many of them."""
+    (L, D), u, m = k.shape, 2.0 ** -24, (k.shape[0] - n + np.arange(n) + (1 if attend_current else 0))[:, None]
+    if L == 0 or n == 0:
+        return np.zeros((n, D)), np.ones(n), np.zeros((n, D)), np.zeros(n)
+    sees = np.arange(L)[None] < m
+    x = np.where(sees, (q @ k.T) * inv_temp, 0.0)
+    ex = 2 * (D + 4) * u * np.where(sees, np.abs(q) @ np.abs(k).T, 0.0).max(1, keepdims=True) * abs(inv_temp)
+    soft = np.where(sees, np.maximum(x, 0) + np.log1p(np.exp(-np.abs(x))), 0.0)
+    total = soft.sum(1, keepdims=True)
+    right = np.cumsum(soft[:, ::-1], 1)[:, ::-1] - soft
+    beta = np.where(sees, 1 / (1 + np.exp(-x)), 0.0)
+    mass = beta.sum(1, keepdims=True)
+    a, rem, some = beta * np.exp(-right), np.exp(-total), m > 0
+    with np.errstate(invalid="ignore", over="ignore"):
+        off = np.minimum(1.0, np.expm1(ex * (1 + mass) + u * (64 + (m / 32 + 8) * right)) + (2.0 ** (-8 * wide) * 1.01 + 8 * m * u if wide else 0))
+        tr = np.where(some, rem * np.minimum(1.0, np.expm1(ex * mass + u * (64 + (m / 32 + 8) * total)) + (8 * m * u if wide else 0)), 0.0)
+    to = (a * off) @ np.abs(v) + 2 * (m / 32 + 40) * u * (a @ np.abs(v))
+    if wide:
+        top = np.maximum.accumulate(np.abs(v), 0)[np.maximum(m[:, 0], 1) - 1]
+        to, tr = to + np.where(some, 2.0 ** -29 * top, 0.0), tr + np.where(some, 2.0 ** -29, 0.0)
+    o, rem, tr = a @ v, rem[:, 0], tr[:, 0]
+    if own_v is not None:
+        o, to = o + rem[:, None] * own_v, to + tr[:, None] * np.abs(own_v)
+    return o, rem, to, tr
+
+
+def tiles_of_blocks(lengths, new, kv, shared, blocks, attend_current=False, tile=256, step=128, cost=2):
+    """How the kernel for many queries deals its tiles to `blocks` blocks: per block, in order, (columns, steps that the block does) of every tile."""
+    see = 1 if attend_current else 0
+    jobs = []  # (columns, steps, steps of keys that the tile does not see)
+    for length, n in zip(lengths, new):
+        steps = max(1, -(-(length - 1 + see) // step))
+        for _ in range(kv):
+            for c0 in range(0, n * shared, tile):
+                cols = min(tile, n * shared - c0)
+                keys = length - n + (c0 + cols - 1) // shared + see
+                jobs.append((cols, steps, steps - max(1, -(-keys // step))))
+    units = sum(s + cost for _, s, _ in jobs)
+    shares = max(1, min(blocks, units))
+    out, at = [[] for _ in range(shares)], 0
+    for cols, steps, unseen in jobs:
+        first, last = at, at + steps + cost
+        at = last
+        for b in range(first * shares // units, shares):
+            lo, hi = max(first, units * b // shares), min(last, units * (b + 1) // shares)
+            if lo >= last:
+                break
+            if lo < hi:
+                out[b].append((cols, max(0, max(0, hi - first - cost) - max(max(0, lo - first - cost), unseen))))
+    return out

@@ -43,6 +43,14 @@ constexpr int kTile = 256, kStep = 128;  // queries of a tile, keys of a step
 constexpr int kJobCost = 2;              // steps that a job costs besides its own
 constexpr uint32_t kTmemCols = 512, kColS = 0, kColO = 256, kColP = 64;
 constexpr int kScaleSlots = 4;
+// Who waits for which use of a barrier.  A wait names a phase by its parity alone: it is right where the barrier has completed all uses before the one that is meant,
+// and at most that one.
+//   Q_FULL (a use per job, two in turn), Q_EMPTY, K_*, RAW_*, READ_*, V_*: converters and the issuing warp go through every job and every step, in order.
+//   S_READY, P_HALF, P_READY, O_READY, O_FREE of a half: used only by jobs that have columns in that half; whoever uses them counts those uses.
+//   SC_FULL (a use per step, four in turn) and Q_FULL as the rows see them: rows of the second half pass over jobs of at most 128 columns without a wait, any number
+//   of them, and would find either barrier uses behind.  So they wait for their scores first.  Scores of step s of job j are issued when the queries of j and the keys of s are there and
+//   the products of step s - 1 have been issued, which had that step's values, scales and all before them.  And until these rows have given the weights of
+//   step s, the scores of s + 2 are not issued, so that no scales of s + 4 and no queries of j + 2 have come.
 enum Bar { Q_FULL0, Q_FULL1, Q_EMPTY, K_FULL, K_EMPTY, RAW_K, RAW_V, READ_K, READ_V, V_FULL0, V_FULL1, V_EMPTY0, V_EMPTY1, SC_FULL0, SC_FULL1, SC_FULL2, SC_FULL3,
            S_READY0, S_READY1, P_READY0, P_READY1, P_HALF0, P_HALF1, O_READY0, O_READY1, O_FREE0, O_FREE1, kNumBars };
 
@@ -462,14 +470,17 @@ __global__ void __launch_bounds__(kThreads, 1) cached_tc_kernel(const __grid_con
             float W = 1.f;
             bool nans = false;
             if (live) {
-                ok = mbar_wait(&sm.bars[Q_FULL0 + (jobs & 1)], (jobs >> 1) & 1, abort_flag);
-                if (!ok) break;
-                const float temp = sm.temp[jobs & 1][c];
+                float temp = 0.f;
                 const int lim = mine ? k.sees(j, c) : 0, least = k.sees(j, 128 * half);
                 for (int pos = first; pos < j.end; ++pos, ++step) {
                     const int key0 = kStep * (j.steps - 1 - pos), slot = step % kScaleSlots;
-                    ok = mbar_wait(&sm.bars[SC_FULL0 + slot], (step / kScaleSlots) & 1, abort_flag) && mbar_wait(&sm.bars[S_READY0 + half], ph_s, abort_flag);
+                    // the scores first: with them, and not before, the two barriers that a half without columns skips are at the use that is meant
+                    ok = mbar_wait(&sm.bars[S_READY0 + half], ph_s, abort_flag) && mbar_wait(&sm.bars[SC_FULL0 + slot], (step / kScaleSlots) & 1, abort_flag);
                     ph_s ^= 1;
+                    if (ok && pos == first) {
+                        ok = mbar_wait(&sm.bars[Q_FULL0 + (jobs & 1)], (jobs >> 1) & 1, abort_flag);
+                        temp = sm.temp[jobs & 1][c];
+                    }
                     if (!ok) break;
                     tc_fence_after();
                     const bool masked = key0 + kStep > least;

@@ -122,3 +122,25 @@ def test_refused_without_cuda():
     for bad in (dict(head_dim=129), dict(head_dim=0), dict(page_tokens=48)):
         with pytest.raises(ValueError):
             sb_cache(**{**dict(pages=2, heads=2, head_dim=50, page_tokens=16, device="cpu"), **bad})
+
+
+@pytest.mark.parametrize("wide", [0, 1, 2])
+@pytest.mark.parametrize("current", [False, True])
+def test_oracle_rows(wide, current):
+    """The oracle of all rows at once is the one of single rows."""
+    rng = np.random.default_rng(wide)
+    for L, n in ((1, 1), (40, 7), (9, 9), (130, 1)):
+        q, k, v, own = (rng.normal(0, 2, (x, 20)) for x in (n, L, L, n))
+        for a, b in zip(orc.attend(q, k, v, n, 0.3, current, own, wide), orc.attend_rows(q, k, v, n, 0.3, current, own, wide)):
+            assert a.shape == b.shape and np.allclose(a, b, rtol=1e-9, atol=1e-300)
+
+
+def test_oracle_tiles():
+    """Every step of every tile is dealt to one block, in order."""
+    lengths, new = [1000, 1, 300, 90, 4000], [70, 1, 300, 0, 33]
+    for blocks in (1, 3, 7, 148):
+        dealt = orc.tiles_of_blocks(lengths, new, 3, 4, blocks)
+        assert len(dealt) == blocks
+        for tile in (256, 128):
+            steps = sum(max(1, -(-(t - n + (min(c + tile, 4 * n) - 1) // 4) // 128)) for t, n in zip(lengths, new) for c in range(0, 4 * n, tile)) * 3
+            assert sum(s for b in orc.tiles_of_blocks(lengths, new, 3, 4, blocks, tile=tile) for _, s in b) == steps

@@ -1,0 +1,101 @@
+"""Attention over the 8-bit paged cache, many queries per key: blocks that go from tile to tile of different widths."""
+import numpy as np
+import pytest
+import torch
+
+from oracle import cache_oracle as orc
+from test_gpu_cache import Problem
+
+pytestmark = pytest.mark.gpu
+
+
+class Rows(Problem):
+    """A Problem whose oracle works on all rows of a request and head at once."""
+
+    def want(self, inv_temp=None, attend_current=False, v=None, wide=False):
+        inv_temp = self.dim ** -0.5 if inv_temp is None else inv_temp
+        q = self.q.double().cpu().numpy()
+        own = v.double().cpu().numpy() if v is not None else None
+        terms = (2 if self.q.dtype == torch.float16 else 1) if wide else 0
+        shared, outs, at = self.heads // self.kv, [[], [], [], []], 0
+        for r, n in enumerate(self.new):
+            rows = slice(at, at + n)
+            at += n
+            per = [orc.attend_rows(q[h, rows], self.k[r][h // shared], self.v[r][h // shared], n, inv_temp, attend_current, own[h // shared, rows] if own is not None else None, terms)
+                   for h in range(self.heads)]
+            for out, x in zip(outs, zip(*per)):
+                out.append(np.stack(x))
+        return [np.concatenate(x, 1) for x in outs]
+
+    def other_powers(self):
+        """Queries whose largest values lie in different powers of two from request to request, at the same logits."""
+        at = 0
+        for r, n in enumerate(self.new):
+            e = r * 5 % 13 - 6
+            self.q[:, at:at + n] *= 2.0 ** e
+            self.k[r] *= 2.0 ** -e
+            pages = self.tables[r][self.tables[r] >= 0]
+            self.cache.k_scale[torch.tensor(pages, device="cuda")] *= 2.0 ** -e
+            at += n
+        return self
+
+
+def sms():
+    return torch.cuda.get_device_properties(0).multi_processor_count
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("dim, page", [(128, 64), (64, 16), (32, 32)])
+def test_narrow_tiles_before_full_ones(dim, page, dtype):
+    """Tiles of at most 128 columns, whose second half of rows has nothing to do, one behind the other before a tile that has work for it: 2 to 5 and more of them, the full tile
+    at every number of jobs modulo four (tiles' queries have two places in turn, their marks four).  Logits are of order one; factors of
+    queries differ from request to request, so that those of another tile give other results."""
+    rng = np.random.default_rng(dim)
+    count = 13 * sms() // 8  # about thirteen tiles a block
+    lengths = [int(x) for x in rng.integers(64, 129, count)]
+    lengths[::9] = [x + 200 for x in lengths[::9]]
+    new = [int(rng.integers(1, 33)) if r % 2 else 64 for r in range(count)]  # 4 ... 128 columns, or 256
+    p = Rows(lengths, new, heads=32, kv=8, dim=dim, page=page, dtype=dtype, lean=2.0, seed=dim).other_powers()
+    runs, places = set(), set()
+    for tiles in orc.tiles_of_blocks(lengths, new, 8, 4, sms()):
+        run = 0
+        for i, (cols, steps) in enumerate(t for t in tiles if t[1] > 0):
+            if cols > 128 and run > 1:
+                runs.add(run)
+                places.add(i % 4)
+            run = run + 1 if cols <= 128 else 0
+    assert {2, 3, 4, 5} <= runs and places == {0, 1, 2, 3}
+    p.check(v=p.own_v, wide=True)
+
+
+@pytest.mark.parametrize("lengths, new", [([1000] * 64, [20, 200] * 32), ([2000] * 64, [1] * 7 + [512])])
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_single_tokens_beside_prompt_pieces(lengths, new, dtype):
+    """A step of a server: some requests bring one token or a few, others the next piece of a prompt.  Against the same requests one kind at a time, which
+    no tile of the other kind stands beside: the same weights in other shares, which changes float32 sums and the rounding of a few results."""
+    from stickbreaking_attention_b200 import sb_attn_cached, SbCache
+    new = (new * 64)[:64]
+    kv, dim, page, T = 8, 128, 64, sum(new)
+    g = torch.Generator(device="cuda").manual_seed(5)
+    held = -(-lengths[0] // page)
+    normal = lambda *shape: torch.randn(shape, generator=g, device="cuda")  # noqa: E731
+    codes = [normal(64 * held, kv, page, dim).mul_(60).clamp_(-448, 448).to(torch.float8_e4m3fn) for _ in range(2)]
+    scales = [torch.full((64 * held, kv), 2.0 ** -6, device="cuda") for _ in range(2)]
+    cache = SbCache(*codes, *scales)
+    tables = torch.randperm(64 * held, generator=g, device="cuda").int().view(64, held)
+    q = normal(4 * kv, T, dim).to(torch.bfloat16 if dtype == "bf16" else torch.float16)
+    n = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    ends = np.cumsum(new)
+    o, rem = sb_attn_cached(q, cache, tables, n, torch.tensor(ends, dtype=torch.int32, device="cuda"))
+    for kind in sorted(set(new)):
+        pick = [r for r in range(64) if new[r] == kind]
+        rows = torch.cat([torch.arange(ends[r] - new[r], ends[r]) for r in pick]).cuda()
+        at = torch.tensor(pick, device="cuda")
+        mine = torch.tensor(np.cumsum([kind] * len(pick)), dtype=torch.int32, device="cuda")
+        wo, wrem = sb_attn_cached(q[:, rows], cache, tables[at], n[at], mine)
+        # two results of one number, each rounded to the type; on either side weights may have been rounded to a bfloat16 term, 2^-8 of the sum of
+        # |weight * value|, which is at most the largest |value|; eight roundings of 2^-24 a key for the products of 1 - beta
+        top = 448 * 2.0 ** -6
+        half = torch.finfo(q.dtype).eps / 2
+        assert ((o[:, rows].double() - wo.double()).abs() <= 2 * half * wo.double().abs() * (1 + half) + 2 * top * (2.0 ** -8 + 2000 * 8 * 2.0 ** -24)).all()
+        assert ((rem[:, rows].double() - wrem.double()).abs() <= 2 * half * wrem.double() * (1 + half) + 2 * (2000 * 8 * 2.0 ** -24 * wrem.double() + 2.0 ** -29)).all()
