@@ -9,8 +9,8 @@
 // differ from page to page: two bfloat16 terms (2^-16) instead, which the tensor cores, busy a third of the time, multiply one after the other.
 //
 // With e = 2^x and d = 1 + e, 1 - beta = 1 / d.  A thread owns a query; for a group of four keys entered with W, the product of 1 - beta to its right,
-// the weight of key m is e_m (product of d to its left in the group) W / (product of d of the group): one reciprocal per four keys.
-// x is clamped at 30 (1 - beta = 2^-30), so that the product of a group stays below 2^121.
+// the weight of key m is e_m (product of d to its left in the group) / (product of d of the group) W: one reciprocal per four keys.
+// x is clamped at 30 (1 - beta = 2^-30), so that the product of a group stays below 2^121 and its reciprocal a normal number.
 //
 // Warps of a block (512 threads, 128 registers): 0-3 / 4-7 row warps of the first / second half, 8-11 / 12-14 convert the codes of the values / keys, which
 // TMA brings to shared memory a step ahead, all of them the queries, 15 issues tcgen05.mma.
@@ -91,24 +91,27 @@ __device__ __forceinline__ void sweep(const uint32_t (&s)[16], float scale, int 
         }
     }
 }
-// from right to left: the factor of every group; W <- what leaves the 16 keys on their left
-__device__ __forceinline__ void carries(const float2 (&run)[2], float& W, float2 (&f)[2]) {
-#pragma unroll
-    for (int h = 1; h >= 0; --h) {
-        f[h].y = W * rcp_approx(run[h].y);
-        f[h].x = f[h].y * rcp_approx(run[h].x);
-        W = f[h].x;
-    }
+// for every group 1 / (product of d), and W vs as it enters, from right to left; W <- what leaves the 16 keys on their left.  1 / (product of d) may be as small as
+// 2^-120: made one factor with W it would be lost, and with it all of the stick that the group takes.  (W itself underflows where the weights
+// behind it are below 2^-126.)  One factor per group, which this had been, took 195 us where it takes 198 (4 requests of 2000 ... 5000 tokens, below), 152 for 159 at head dim 32.
+__device__ __forceinline__ void carries(const float2 (&run)[2], float vs, float& W, float2 (&r)[2], float2 (&g)[2]) {
+    r[1] = make_float2(rcp_approx(run[1].x), rcp_approx(run[1].y));
+    r[0] = make_float2(rcp_approx(run[0].x), rcp_approx(run[0].y));
+    g[1].y = W * vs;
+    g[1].x = g[1].y * r[1].y;
+    g[0].y = g[1].x * r[1].x;
+    g[0].x = g[0].y * r[0].y;
+    const float2 all = __fmul2_rn(r[0], r[1]);
+    W *= all.x * all.y;
 }
 // kTwo: into two bfloat16 terms, w the leading one
 template <bool kTwo>
-__device__ __forceinline__ void finish(const float2 (&p)[2][4], const float2 (&f)[2], float vs, uint32_t (&w)[8], uint32_t (&low)[8]) {
-    const float2 v = make_float2(vs, vs);  // not into f, which may be as small as 2^-120
+__device__ __forceinline__ void finish(const float2 (&p)[2][4], const float2 (&r)[2], const float2 (&g)[2], uint32_t (&w)[8], uint32_t (&low)[8]) {
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int m = 0; m < 4; m += 2) {
-            const float2 a = __fmul2_rn(__fmul2_rn(p[h][m], f[h]), v), b = __fmul2_rn(__fmul2_rn(p[h][m + 1], f[h]), v);
+            const float2 a = __fmul2_rn(__fmul2_rn(p[h][m], r[h]), g[h]), b = __fmul2_rn(__fmul2_rn(p[h][m + 1], r[h]), g[h]);  // the first product is at most one
             w[4 * h + m / 2] = pack_bf16(a.x, b.x);
             w[4 * h + 2 + m / 2] = pack_bf16(a.y, b.y);
             if (kTwo) {
@@ -137,14 +140,14 @@ __device__ __forceinline__ constexpr int weights_at(int ch) { return kTwo ? 16 *
 template <bool kTwo, bool kMasked>
 __device__ __forceinline__ void row_step(uint32_t s_base, uint64_t* half_ready, const float* ks, const float* vs, float temp, int key0, int lim, float& W) {
     uint32_t u[2][16], w[8], low[8];
-    float2 pw[2][2][4], run[2][2], f[2];
+    float2 pw[2][2][4], run[2][2], r[2], g[2];
     const auto swept = [&](int b, int ch) {
         tmem_wait_ld(u[b]);
         sweep<kMasked>(u[b], ks[ch] * temp, key0 + 16 * ch, lim, pw[b], run[b]);
     };
     const auto out = [&](int b, int ch) {
-        carries(run[b], W, f);
-        finish<kTwo>(pw[b], f, vs[ch], w, low);
+        carries(run[b], vs[ch], W, r, g);
+        finish<kTwo>(pw[b], r, g, w, low);
         tmem_st8(s_base + weights_at<kTwo>(ch), w);
         if (kTwo) tmem_st8(s_base + weights_at<kTwo>(ch) + 8, low);
     };
@@ -511,21 +514,21 @@ __global__ void __launch_bounds__(kThreads, 1) cached_tc_kernel(const __grid_con
             if (mine && whole) k.template store<1>(j, c, p.head_dim, {0.f}, sum, true);  // rem alone
             if (mine && !whole) slot[kTile * ROW + c] = sum;
 #pragma unroll 1
-            for (int d0 = 0; d0 < ROW; d0 += 32) {
-                uint32_t v[32];
+            for (int d0 = 0; d0 < ROW; d0 += 16) {  // 32 columns at a time: 1 to 3 % more, the steps' registers suffer
+                uint32_t v[16];
                 if (live) {
-                    tmem_ld32(o_base + d0, v);
+                    tmem_ld16(o_base + d0, v);
                     tmem_wait_ld(v);
                 } else {
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) v[i] = 0u;
+                    for (int i = 0; i < 16; ++i) v[i] = 0u;
                 }
-                if (live && d0 + 32 == ROW) {
+                if (live && d0 + 16 == ROW) {
                     tc_fence_before();
                     mbar_arrive(&sm.bars[O_FREE0 + half]);
                 }
                 if (!mine) continue;
-                float (&x)[32] = *(float (*)[32]) & v;
+                float (&x)[16] = *(float (*)[16]) & v;
                 if (nans) {  // rare: NaN in a value that this query sees
                     const int lim = k.sees(j, c);
                     for (int key = max(k.sees(j, 0), kStep * (j.steps - j.end)); key < min(lim, kStep * (j.steps - first)); ++key) {
@@ -533,15 +536,15 @@ __global__ void __launch_bounds__(kThreads, 1) cached_tc_kernel(const __grid_con
                         if (page < 0 || page >= p.pages) continue;
                         const uint8_t* code = (const uint8_t*)p.v_codes + page * p.v_stride + ((int64_t)j.g * P + key % P) * ROW + d0;
 #pragma unroll
-                        for (int i = 0; i < 32; ++i)
+                        for (int i = 0; i < 16; ++i)
                             if ((code[i] & 127) == 127) x[i] = __int_as_float(0x7fc00000);
                     }
                 }
                 if (whole) {
-                    k.template store<32>(j, c, d0, x, sum, false);
+                    k.template store<16>(j, c, d0, x, sum, false);
                 } else {
 #pragma unroll
-                    for (int i = 0; i < 32; i += 4) *(float4*)(slot + c * ROW + d0 + i) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
+                    for (int i = 0; i < 16; i += 4) *(float4*)(slot + c * ROW + d0 + i) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
                 }
             }
             if (n > 0) ++jobs;

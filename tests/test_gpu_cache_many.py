@@ -99,3 +99,41 @@ def test_single_tokens_beside_prompt_pieces(lengths, new, dtype):
         half = torch.finfo(q.dtype).eps / 2
         assert ((o[:, rows].double() - wo.double()).abs() <= 2 * half * wo.double().abs() * (1 + half) + 2 * top * (2.0 ** -8 + 2000 * 8 * 2.0 ** -24)).all()
         assert ((rem[:, rows].double() - wrem.double()).abs() <= 2 * half * wrem.double() * (1 + half) + 2 * (2000 * 8 * 2.0 ** -24 * wrem.double() + 2.0 ** -29)).all()
+
+
+# ------------------------------------------------------------------------------------------------------ weights
+def built(logits, length, new, value_at, dtype, dim=64, page=16):
+    """One request whose keys have the given logits (e4m3 values; -16 elsewhere) for every query, and a value of one at `value_at`, zero elsewhere."""
+    p = Rows([length], [new], heads=2, kv=1, dim=dim, page=page, dtype=dtype).widen()
+    x = np.full(length, -16.0)
+    for key, t in logits.items():
+        x[key] = t
+    p.k, p.v = [np.zeros((1, length, dim))], [np.zeros((1, length, dim))]
+    p.k[0][0, :, 0] = x
+    p.v[0][0, value_at, 0] = p.v[0][0, value_at, 1] = 1.0
+    for codes, scales, y in ((p.cache.k, p.cache.k_scale, p.k[0]), (p.cache.v, p.cache.v_scale, p.v[0])):
+        scales.fill_(1.0)
+        for b in range(-(-length // page)):
+            n = min(page, length - b * page)
+            codes.view(torch.uint8)[int(p.tables[0, b]), 0, :n] = torch.tensor(orc.to_code(y[0, b * page:b * page + n]), device="cuda")
+    p.q.zero_()
+    p.q[..., 0] = 1.0
+    return p
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("first", [36, 40, 44, 48, 260, 264, 268, 272])
+@pytest.mark.parametrize("logit", [5.0, 6.0, 10.0, 14.0, 18.0])
+def test_strong_keys_behind_a_stick_that_is_partly_used(first, logit, dtype):
+    """Four neighbouring keys whose logits pass the clamp of 1 - beta, with a key to their right that leaves 2^-7 to 2^-26 of the stick: the rightmost of the four takes
+    all of that, and nothing of it may be lost to products of 1 + e that leave float32's range.  In steps that all queries see, and in the one that some do."""
+    built({**{first + i: 24.0 for i in range(4)}, first + 5: logit}, 300, 40, first + 3, dtype).check(inv_temp=1.0, wide=True)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_strong_keys_one_behind_the_other(dtype):
+    """Strong and middling keys at every place of a group: each takes its part of what the ones to its right have left."""
+    for shift in range(4):
+        logits = {100 + shift + i: t for i, t in enumerate([22.0, 4.0, 24.0, 1.0, 3.5, 20.0, 2.0, 0.5, 6.0, 5.0, 3.0])}
+        for at in (100 + shift, 103 + shift, 105 + shift, 108 + shift):
+            built(logits, 300, 40, at, dtype).check(inv_temp=1.0, wide=True)
