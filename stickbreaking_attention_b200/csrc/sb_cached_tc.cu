@@ -4,9 +4,10 @@
 // A tile is two halves of 128 queries (rows of tensor memory) against the same keys, which take turns as in sb_tc_fwd_pair.cu: while the row threads of
 // one turn scores into weights, the tensor cores work for the other.  Codes become 16-bit operands once per block and step: keys float16 (exact; the queries
 // are scaled by a power of two per row to at most 2^15, exact too), values bfloat16 (exact).  The scale of the keys' page goes into the factor of a
-// score, that of the values' page into the weight before it is rounded to bfloat16: one rounding of the weights, as in the forward
-// kernels, and bfloat16's range.  For float16 one rounding to bfloat16 would be eight of its own, and float16 weights would lack the range for scales that
-// differ from page to page: two bfloat16 terms (2^-16) instead, which the tensor cores, busy a third of the time, multiply one after the other.
+// score, that of the values' page into the weight before that becomes two bfloat16 terms (2^-16 of it is lost; float16 weights would lack the range for scales
+// that differ from page to page), which the tensor cores multiply one after the other.  One term would do for bfloat16 results if all came from this kernel, as in
+// the forward kernels, and takes 198 us for 219 (below); but the same request comes here or to sb_cached.cu by what its batch looks like, and 2^-8 of the weights show
+// in its results (2-norm 2.4e-3 of float64 for 1.7e-3, the output's own rounding), 2^-16 do not.
 //
 // With e = 2^x and d = 1 + e, 1 - beta = 1 / d.  A thread owns a query; for a group of four keys entered with W, the product of 1 - beta to its right,
 // the weight of key m is e_m (product of d to its left in the group) / (product of d of the group) W: one reciprocal per four keys.
@@ -15,8 +16,7 @@
 // Warps of a block (512 threads, 128 registers): 0-3 / 4-7 row warps of the first / second half, 8-11 / 12-14 convert the codes of the values / keys, which
 // TMA brings to shared memory a step ahead, all of them the queries, 15 issues tcgen05.mma.
 // The product with the values starts with the right 64 keys while rows work on the left ones (173 -> 163 us at head dim 64, 160 -> 152 at 32, nothing at 128).
-// Tensor memory (512 columns): scores of the halves at 0 / 128 (weights overwrite the right half of their scores,
-// two terms the scores of the same keys), sums at 256 / 384.
+// Tensor memory (512 columns): scores of the halves at 0 / 128 (the weights' two terms overwrite the scores of the same keys), sums at 256 / 384.
 //
 // Measured: 4 requests of 2000 ... 5000 tokens, 512 new ones each, 32 heads over 8, head dim 128: 195 us, 577 TFLOP/s (70 us at the rate of a bfloat16 GEMM), where
 // the kernel of sb_cached.cu takes 1 868. The special-function unit needs 2 560 cycles for a step of both halves, which takes about 5 500: issue slots are half busy,
@@ -41,7 +41,7 @@ using bf16 = __nv_bfloat16;
 constexpr int kThreads = 512, kMmaWarp = 15, kConverters = 7, kValueWarps = 4;
 constexpr int kTile = 256, kStep = 128;  // queries of a tile, keys of a step
 constexpr int kJobCost = 2;              // steps that a job costs besides its own
-constexpr uint32_t kTmemCols = 512, kColS = 0, kColO = 256, kColP = 64;
+constexpr uint32_t kTmemCols = 512, kColS = 0, kColO = 256;
 constexpr int kScaleSlots = 4;
 // Who waits for which use of a barrier.  A wait names a phase by its parity alone: it is right where the barrier has completed all uses before the one that is meant,
 // and at most that one.
@@ -59,6 +59,7 @@ struct Small {  // behind the tiles
     float temp[2][kTile];            // of the jobs in turn: inv_temp log2(e) by what the query was multiplied with
     float ks[kScaleSlots][8], vs[kScaleSlots][8];  // of the steps in turn: scales of 16 keys each
     uint32_t nan_job[4];             // of the jobs in turn: 1 + number of the job, if it has NaN among the values of keys that not all of its queries see
+    Job job[8];                      // of the row warps: here, not in registers
     uint32_t tmem, abort;
 };
 
@@ -104,8 +105,7 @@ __device__ __forceinline__ void carries(const float2 (&run)[2], float vs, float&
     const float2 all = __fmul2_rn(r[0], r[1]);
     W *= all.x * all.y;
 }
-// kTwo: into two bfloat16 terms, w the leading one
-template <bool kTwo>
+// into two bfloat16 terms, w the leading one
 __device__ __forceinline__ void finish(const float2 (&p)[2][4], const float2 (&r)[2], const float2 (&g)[2], uint32_t (&w)[8], uint32_t (&low)[8]) {
 #pragma unroll
     for (int h = 0; h < 2; ++h)
@@ -114,11 +114,12 @@ __device__ __forceinline__ void finish(const float2 (&p)[2][4], const float2 (&r
             const float2 a = __fmul2_rn(__fmul2_rn(p[h][m], r[h]), g[h]), b = __fmul2_rn(__fmul2_rn(p[h][m + 1], r[h]), g[h]);  // the first product is at most one
             w[4 * h + m / 2] = pack_bf16(a.x, b.x);
             w[4 * h + 2 + m / 2] = pack_bf16(a.y, b.y);
-            if (kTwo) {
-                const auto rest = [](uint32_t t, float l, float r) { return pack_bf16(l - __uint_as_float(t << 16), r - __uint_as_float(t & 0xffff0000u)); };
-                low[4 * h + m / 2] = rest(w[4 * h + m / 2], a.x, b.x);
-                low[4 * h + 2 + m / 2] = rest(w[4 * h + 2 + m / 2], a.y, b.y);
-            }
+            const uint32_t wx = w[4 * h + m / 2], wy = w[4 * h + 2 + m / 2];
+            const float2 minus = make_float2(-1.f, -1.f);
+            const float2 c = __ffma2_rn(make_float2(__uint_as_float(wx << 16), __uint_as_float(wy << 16)), minus, a);
+            const float2 d = __ffma2_rn(make_float2(__uint_as_float(wx & 0xffff0000u), __uint_as_float(wy & 0xffff0000u)), minus, b);
+            low[4 * h + m / 2] = pack_bf16(c.x, d.x);
+            low[4 * h + 2 + m / 2] = pack_bf16(c.y, d.y);
         }
 }
 __device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
@@ -127,17 +128,13 @@ __device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8])
                  : "memory");
 }
 
-// Columns of 16 keys' weights, from the first column of the scores: the right half of them, or those of the same 16 keys' scores (two terms)
-template <bool kTwo>
-__device__ __forceinline__ constexpr int weights_at(int ch) { return kTwo ? 16 * ch : kColP + 8 * ch; }
-
 // One row of a step, 16 keys at a time from the right, one such group ahead: exponentials of the next keys (special functions) stand beside the weights
 // of these (arithmetic), scores of the keys after them travel.  Weights go to columns of scores that have been read.  A loop, not its rounds one behind
 // the other: the code of all roles has to stay in the instruction cache (12 % of the kernel).  us for 32 keys at a time, all exponentials and then all weights,
-// with spilled registers / this: 4 requests of 4000 tokens, 512 new ones, 32 heads over 8, bfloat16, head dim 128: 213 / 205, 64: 183 / 164, 32: 169 / 152,
+// with spilled registers / this, one term of the weights for bfloat16: 4 requests of 4000 tokens, 512 new ones, 32 heads over 8, bfloat16, head dim 128: 213 / 205, 64: 183 / 164, 32: 169 / 152,
 // float16, 128: 266 / 226.  Jobs of few steps do not gain: 64 requests of 1000 tokens, 8 heads, head dim 128, 512 columns 277 / 276, 32 columns 131 / 131, head dim 32,
 // 64 columns 93 / 96; with masked steps in this form too (twice the code) 285, 137 and 103.  More registers for rows by setmaxnreg did not help the first form.
-template <bool kTwo, bool kMasked>
+template <bool kMasked>
 __device__ __forceinline__ void row_step(uint32_t s_base, uint64_t* half_ready, const float* ks, const float* vs, float temp, int key0, int lim, float& W) {
     uint32_t u[2][16], w[8], low[8];
     float2 pw[2][2][4], run[2][2], r[2], g[2];
@@ -147,9 +144,9 @@ __device__ __forceinline__ void row_step(uint32_t s_base, uint64_t* half_ready, 
     };
     const auto out = [&](int b, int ch) {
         carries(run[b], vs[ch], W, r, g);
-        finish<kTwo>(pw[b], r, g, w, low);
-        tmem_st8(s_base + weights_at<kTwo>(ch), w);
-        if (kTwo) tmem_st8(s_base + weights_at<kTwo>(ch) + 8, low);
+        finish(pw[b], r, g, w, low);
+        tmem_st8(s_base + 16 * ch, w);  // in the columns of the same 16 keys' scores
+        tmem_st8(s_base + 16 * ch + 8, low);
     };
     if (kMasked) {  // few steps of a job: short code counts for more
 #pragma unroll 1
@@ -193,7 +190,7 @@ template <typename T, int ROW>
 __global__ void __launch_bounds__(kThreads, 1) cached_tc_kernel(const __grid_constant__ SbCacheParams p, const __grid_constant__ Plan pl, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
     constexpr int DP = ROW < 64 ? 64 : ROW;
     using J = Jobs<T, ROW, kTile, kStep, kJobCost>;
-    constexpr bool kTwo = std::is_same<T, __half>::value;  // float16: weights in two terms
+    constexpr bool kHalf = std::is_same<T, __half>::value;
     constexpr int kHalfBytes = 128 * DP * 2, kBoxBytes = 128 * 128;
     extern __shared__ __align__(1024) uint8_t smem[];
     uint8_t* const sQ = smem;                       // two halves
@@ -322,14 +319,14 @@ __global__ void __launch_bounds__(kThreads, 1) cached_tc_kernel(const __grid_con
                     float y[8], top = 0.f;
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
-                        if (kTwo) y[i] = __half2float(__ushort_as_half((unsigned short)(x[i >> 1] >> 16 * (i & 1))));
+                        if (kHalf) y[i] = __half2float(__ushort_as_half((unsigned short)(x[i >> 1] >> 16 * (i & 1))));
                         else y[i] = __uint_as_float(i & 1 ? x[i >> 1] & 0xffff0000u : x[i >> 1] << 16);
                         const float a = fabsf(y[i]);
                         if (a <= 3.4028234664e38f) top = fmaxf(top, a);
                     }
 #pragma unroll
                     for (int off = 1; off < kLanes; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-                    const int e = top > 0.f ? min(max((int)(__float_as_uint(top) >> 23) - 127, -112), kTwo ? 14 : 127) : 14;  // up to 2^(e + 1); float16 is never made smaller
+                    const int e = top > 0.f ? min(max((int)(__float_as_uint(top) >> 23) - 127, -112), kHalf ? 14 : 127) : 14;  // up to 2^(e + 1); float16 is never made smaller
                     const float up = pow2(14 - e);
                     *(uint4*)(sQ + (c >> 7) * kHalfBytes + (d >> 6) * kBoxBytes + row * 128 + ((((d >> 3) & 7) ^ (row & 7)) << 4)) =
                         make_uint4(pack_f16(y[0] * up, y[1] * up), pack_f16(y[2] * up, y[3] * up), pack_f16(y[4] * up, y[5] * up), pack_f16(y[6] * up, y[7] * up));
@@ -436,9 +433,9 @@ __global__ void __launch_bounds__(kThreads, 1) cached_tc_kernel(const __grid_con
                             if (!ok) break;
                             tc_fence_after();
                         }
-                        if (i == kStep / 16 - 1) mma_ts_dyn(leader, d, a + weights_at<kTwo>(i), b, i * 2048, idesc_o, s > 0);
-                        else mma_ts<true>(leader, d, a + weights_at<kTwo>(i), b, i * 2048, idesc_o);
-                        if (kTwo) mma_ts<true>(leader, d, a + weights_at<kTwo>(i) + 8, b, i * 2048, idesc_o);
+                        if (i == kStep / 16 - 1) mma_ts_dyn(leader, d, a + 16 * i, b, i * 2048, idesc_o, s > 0);
+                        else mma_ts<true>(leader, d, a + 16 * i, b, i * 2048, idesc_o);
+                        mma_ts<true>(leader, d, a + 16 * i + 8, b, i * 2048, idesc_o);
                     }
                     if (!ok) break;
                     if (t == halves - 1) mma_commit(leader, &sm.bars[V_EMPTY0 + st]);
@@ -472,6 +469,9 @@ __global__ void __launch_bounds__(kThreads, 1) cached_tc_kernel(const __grid_con
             const bool mine = c < j.cols, live = n > 0 && 128 * half < j.cols;
             float W = 1.f;
             bool nans = false;
+            __syncwarp();
+            if (lane == 0) sm.job[warp] = j;
+            __syncwarp();
             if (live) {
                 float temp = 0.f;
                 const int lim = mine ? k.sees(j, c) : 0, least = k.sees(j, 128 * half);
@@ -487,8 +487,8 @@ __global__ void __launch_bounds__(kThreads, 1) cached_tc_kernel(const __grid_con
                     if (!ok) break;
                     tc_fence_after();
                     const bool masked = key0 + kStep > least;
-                    if (masked) row_step<kTwo, true>(s_base, &sm.bars[P_HALF0 + half], sm.ks[slot], sm.vs[slot], temp, key0, lim, W);
-                    else row_step<kTwo, false>(s_base, &sm.bars[P_HALF0 + half], sm.ks[slot], sm.vs[slot], temp, 0, 0, W);
+                    if (masked) row_step<true>(s_base, &sm.bars[P_HALF0 + half], sm.ks[slot], sm.vs[slot], temp, key0, lim, W);
+                    else row_step<false>(s_base, &sm.bars[P_HALF0 + half], sm.ks[slot], sm.vs[slot], temp, 0, 0, W);
                     tmem_wait_st();
                     tc_fence_before();
                     mbar_arrive(&sm.bars[P_READY0 + half]);
@@ -496,8 +496,8 @@ __global__ void __launch_bounds__(kThreads, 1) cached_tc_kernel(const __grid_con
                 if (!ok) break;
                 if (mine && p.v.ptr) {  // for the end of the job
                     int h;
-                    const int t = k.row_of(j, c, h);
-                    const char* v = (const char*)p.v.ptr + 2 * (j.g * p.v.stride_h + t * p.v.stride_t);
+                    const int t = k.row_of(sm.job[warp], c, h);
+                    const char* v = (const char*)p.v.ptr + 2 * (sm.job[warp].g * p.v.stride_h + t * p.v.stride_t);
                     for (int b = 0; b < 2 * p.head_dim; b += 128) asm volatile("prefetch.global.L1 [%0];" ::"l"(v + b));
                 }
                 ok = mbar_wait(&sm.bars[O_READY0 + half], ph_o, abort_flag);
@@ -508,10 +508,11 @@ __global__ void __launch_bounds__(kThreads, 1) cached_tc_kernel(const __grid_con
             } else {
                 step += n;
             }
-            const bool starts_here = j.starts, whole = j.starts && j.ends;
+            const Job e = sm.job[warp];
+            const bool starts_here = e.starts, whole = e.starts && e.ends;
             float* const slot = pl.slots + ((size_t)self * 2 + (starts_here ? 1 : 0)) * slot_floats(kTile, ROW);
             const float sum = -lg2_approx(W);
-            if (mine && whole) k.template store<1>(j, c, p.head_dim, {0.f}, sum, true);  // rem alone
+            if (mine && whole) k.template store<1>(e, c, p.head_dim, {0.f}, sum, true);  // rem alone
             if (mine && !whole) slot[kTile * ROW + c] = sum;
 #pragma unroll 1
             for (int d0 = 0; d0 < ROW; d0 += 16) {  // 32 columns at a time: 1 to 3 % more, the steps' registers suffer
@@ -530,18 +531,18 @@ __global__ void __launch_bounds__(kThreads, 1) cached_tc_kernel(const __grid_con
                 if (!mine) continue;
                 float (&x)[16] = *(float (*)[16]) & v;
                 if (nans) {  // rare: NaN in a value that this query sees
-                    const int lim = k.sees(j, c);
-                    for (int key = max(k.sees(j, 0), kStep * (j.steps - j.end)); key < min(lim, kStep * (j.steps - first)); ++key) {
-                        const int page = p.tables[j.r * p.table_stride + key / P];
+                    const int lim = k.sees(e, c);
+                    for (int key = max(k.sees(e, 0), kStep * (e.steps - e.end)); key < min(lim, kStep * (e.steps - first)); ++key) {
+                        const int page = p.tables[e.r * p.table_stride + key / P];
                         if (page < 0 || page >= p.pages) continue;
-                        const uint8_t* code = (const uint8_t*)p.v_codes + page * p.v_stride + ((int64_t)j.g * P + key % P) * ROW + d0;
+                        const uint8_t* code = (const uint8_t*)p.v_codes + page * p.v_stride + ((int64_t)e.g * P + key % P) * ROW + d0;
 #pragma unroll
                         for (int i = 0; i < 16; ++i)
                             if ((code[i] & 127) == 127) x[i] = __int_as_float(0x7fc00000);
                     }
                 }
                 if (whole) {
-                    k.template store<16>(j, c, d0, x, sum, false);
+                    k.template store<16>(e, c, d0, x, sum, false);
                 } else {
 #pragma unroll
                     for (int i = 0; i < 16; i += 4) *(float4*)(slot + c * ROW + d0 + i) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);

@@ -16,7 +16,7 @@ class Rows(Problem):
         inv_temp = self.dim ** -0.5 if inv_temp is None else inv_temp
         q = self.q.double().cpu().numpy()
         own = v.double().cpu().numpy() if v is not None else None
-        terms = (2 if self.q.dtype == torch.float16 else 1) if wide else 0
+        terms = 2 if wide else 0  # of bfloat16, for the weights
         shared, outs, at = self.heads // self.kv, [[], [], [], []], 0
         for r, n in enumerate(self.new):
             rows = slice(at, at + n)
@@ -137,3 +137,12 @@ def test_strong_keys_one_behind_the_other(dtype):
         logits = {100 + shift + i: t for i, t in enumerate([22.0, 4.0, 24.0, 1.0, 3.5, 20.0, 2.0, 0.5, 6.0, 5.0, 3.0])}
         for at in (100 + shift, 103 + shift, 105 + shift, 108 + shift):
             built(logits, 300, 40, at, dtype).check(inv_temp=1.0, wide=True)
+
+
+@pytest.mark.parametrize("dim, page", [(128, 64), (64, 16), (32, 32)])
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_weights_keep_sixteen_bits(dim, page, dtype):
+    """A prompt piece gets the weights that single tokens get but for 2^-16 of them, whatever type its queries have: what is left is the rounding of the results."""
+    p = Rows([300, 700, 150], [64, 200, 90], heads=8, kv=2, dim=dim, page=page, dtype=dtype, lean=3.0, seed=dim).widen()
+    p.check(wide=True)
+    p.check(attend_current=True, v=p.own_v, wide=True)
