@@ -12,8 +12,9 @@ BINDING = os.path.join(HERE, "_binding.so")
 BINDING_SRC = os.path.join(HERE, "csrc", "sb_torch.cpp")
 FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17", "--use_fast_math",
          "-Xcompiler", "-fPIC"]
-# the kernels of float32 precision, which need accurate exponentials, denormal numbers and IEEE division: compiled without --use_fast_math
-PRECISE = {"sb_f32.cu", "sb_f32_tc.cu", "sb_weights.cu", "sb_cache_append.cu", "sb_cached.cu"}
+# the kernels of float32 precision, which need accurate exponentials, denormal numbers and IEEE division, and those of the cache, whose scales bring small numbers
+# back (sb_cached_tc.cu: queries below 2^-112 under keys of large scales; not slower by it): compiled without --use_fast_math
+PRECISE = {"sb_f32.cu", "sb_f32_tc.cu", "sb_weights.cu", "sb_cache_append.cu", "sb_cached.cu", "sb_cached_tc.cu"}
 
 
 def sources():

@@ -146,3 +146,18 @@ def test_weights_keep_sixteen_bits(dim, page, dtype):
     p = Rows([300, 700, 150], [64, 200, 90], heads=8, kv=2, dim=dim, page=page, dtype=dtype, lean=3.0, seed=dim).widen()
     p.check(wide=True)
     p.check(attend_current=True, v=p.own_v, wide=True)
+
+
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("queries", [-129, -118, -60, 60, 105])
+def test_bfloat16_range(queries, wide):
+    """Queries at both ends of bfloat16, subnormal ones among them, and keys whose scales bring the logits back to order one."""
+    p = Rows([300, 150], [100, 90] if wide else [3, 1], heads=4, kv=2, dim=64, page=16, dtype="bf16", lean=1.0, seed=6)
+    if wide:
+        p.widen()
+    keys = min(-queries, 124)  # the largest scale is 2^118: 448 times it is still a float32 number
+    p.q = (p.q.double() * 2.0 ** queries).to(torch.bfloat16)
+    for r in range(2):
+        p.k[r] *= 2.0 ** keys
+    p.cache.k_scale.mul_(2.0 ** keys)
+    p.check(inv_temp=2.0 ** (-3 - queries - keys), wide=wide)
