@@ -21,8 +21,6 @@ __device__ inline float scale_for(float a) {
     e = max(e, kScaleMinExp);
     return __uint_as_float((uint32_t)(e + 127) << 23);
 }
-// 1 / s of a power of two between 2^-126 and 2^126
-__device__ inline float inverse_pow2(float s) { return __uint_as_float((254u << 23) - __float_as_uint(s)); }
 
 // the code of a float32 number that is at most 448 in magnitude; NaN code for infinities and NaN
 __device__ inline uint8_t to_e4m3(float x) {
