@@ -161,3 +161,47 @@ def test_bfloat16_range(queries, wide):
         p.k[r] *= 2.0 ** keys
     p.cache.k_scale.mul_(2.0 ** keys)
     p.check(inv_temp=2.0 ** (-3 - queries - keys), wide=wide)
+
+
+def narrow_and_full(dtype, dim=64, page=16, kv=8):
+    rng = np.random.default_rng(3)
+    count = 13 * sms() // 8
+    lengths = [int(x) for x in rng.integers(64, 129, count)]
+    new = [int(rng.integers(1, 33)) if r % 3 else 64 for r in range(count)]
+    return Rows(lengths, new, heads=4 * kv, kv=kv, dim=dim, page=page, dtype=dtype, lean=2.0, seed=4).other_powers()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_tiles_of_different_widths_give_the_same_bits_every_time(dtype):
+    """Calls that overlap on several streams."""
+    from stickbreaking_attention_b200 import sb_attn_cached
+    p = narrow_and_full(dtype)
+    first = p.run(v=p.own_v)
+    t, n, ends = (torch.tensor(np.ascontiguousarray(x), dtype=torch.int32, device="cuda") for x in (p.tables, p.lengths, np.cumsum(p.new)))
+    call = lambda: sb_attn_cached(p.q, p.cache, t, n, ends, v=p.own_v)  # noqa: E731
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    torch.cuda.synchronize()
+    outs = []
+    for i in range(12):
+        with torch.cuda.stream(streams[i % 3]):
+            outs.append(call())
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for out in outs for a, b in zip(out, first))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_nan_in_one_tile_of_many(dtype):
+    """NaN in values that some queries of a tile see, in tiles of many, narrow and full: the results of those queries, in that column, and no others."""
+    p = narrow_and_full(dtype)
+    clean_o, clean_rem = p.run()
+    bad = torch.zeros_like(clean_o, dtype=torch.bool)
+    first = np.cumsum(p.new) - p.new
+    for r in range(1, len(p.lengths), 5):
+        length, n, g = p.lengths[r], p.new[r], r % p.kv
+        key = length - 1 - n // 2  # seen by the rows behind it
+        p.cache.v.view(torch.uint8)[int(p.tables[r, key // p.page]), g, key % p.page, 9] = 127
+        sees = key - (length - n) + 1
+        bad[4 * g:4 * g + 4, first[r] + sees:first[r] + n, 9] = True
+    assert bad.any()
+    o, rem = p.run()
+    assert o[bad].isnan().all() and torch.equal(o[~bad], clean_o[~bad]) and torch.equal(rem, clean_rem)
