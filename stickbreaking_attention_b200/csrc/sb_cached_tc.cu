@@ -94,16 +94,19 @@ __device__ __forceinline__ void sweep(const uint32_t (&s)[16], float scale, int 
 }
 // for every group 1 / (product of d), and W vs as it enters, from right to left; W <- what leaves the 16 keys on their left.  1 / (product of d) may be as small as
 // 2^-120: made one factor with W it would be lost, and with it all of the stick that the group takes.  (W itself underflows where the weights
-// behind it are below 2^-126.)  One factor per group, which this had been, took 195 us where it takes 198 (4 requests of 2000 ... 5000 tokens, below), 152 for 159 at head dim 32.
+// behind it are below 2^-126.)  One factor per group, which this had been, took 195 us where two take 198 (4 requests of 2000 ... 5000 tokens, below; weights in one
+// term), 152 for 159 at head dim 32.  W goes from group to group: by the product of the four reciprocals it loses 2.7e-4 of itself over 60 000 tokens for 2.0e-4 (the
+// reciprocal is on average 1e-8 too small), for the same time; reciprocals put right by a Newton step leave 1e-5 and cost 2 to 5 %.
 __device__ __forceinline__ void carries(const float2 (&run)[2], float vs, float& W, float2 (&r)[2], float2 (&g)[2]) {
     r[1] = make_float2(rcp_approx(run[1].x), rcp_approx(run[1].y));
     r[0] = make_float2(rcp_approx(run[0].x), rcp_approx(run[0].y));
-    g[1].y = W * vs;
-    g[1].x = g[1].y * r[1].y;
-    g[0].y = g[1].x * r[1].x;
-    g[0].x = g[0].y * r[0].y;
-    const float2 all = __fmul2_rn(r[0], r[1]);
-    W *= all.x * all.y;
+#pragma unroll
+    for (int h = 1; h >= 0; --h) {
+        g[h].y = W * vs;
+        W *= r[h].y;
+        g[h].x = W * vs;
+        W *= r[h].x;
+    }
 }
 // into two bfloat16 terms, w the leading one
 __device__ __forceinline__ void finish(const float2 (&p)[2][4], const float2 (&r)[2], const float2 (&g)[2], uint32_t (&w)[8], uint32_t (&low)[8]) {
