@@ -16,7 +16,7 @@
 //   * a lane forms one key's weight for every column in float32: soft and its sums over the lanes by shuffles, the carry compensated;
 //   * the weights of 32 keys, with the scale of the values' page, are scaled by a power of two to at most 2^15 per column and split into two float16 terms
 //     (22 bits: what is lost is below float32's own rounding of the sums), the two products are added to float32 accumulators.
-// float32 queries are two float16 terms, too; 16-bit ones are scaled by a power of two per row and exact.
+// float32 queries are two float16 terms, too; 16-bit ones are scaled by a power of two per row and exact (bfloat16: elements above 2^-31 of the row's largest).
 //
 // Measured (a copy's bandwidth is 6 551 GB/s): 32 requests of 1000 ... 12 000 tokens, 32 heads, head dim 128, 1.32 GB of codes 228-240 us, 5 500-5 800 GB/s; one request
 // of 65 536 tokens, 8 heads 40 us, of which the steps take 18 (a bandwidth of 7 300 GB/s; what the loads cannot use is the start, lengths, tables, queries, and the
@@ -565,18 +565,19 @@ int launch_row(const SbCacheParams& p, cudaStream_t st) {
 
 // Whether the kernel of sb_cached_tc.cu takes the call: 16-bit types, and enough queries per key on average over the requests.  Both ways, us a call, bfloat16, by
 // queries (heads of a group times new tokens) of a request and key/value head:
-//   16 requests of 2000 tokens, 8 heads, head dim 128      8: 34 / 59   16: 51 / 62   32: 86 / 66   64: 153 / 68   256: 537 / 102   1024: 2055 / 269
-//   64 requests of 1000 tokens, 8 heads, head dim 128      8: 55 / 133  16: 89 / 136  32: 155 / 141  64: 284 / 139  256: 1024 / 194
-//   1 request of 16 000 tokens, 8 heads, head dim 128      8: 42 / 35   16: 42 / 38   32: 53 / 44   64: 82 / 45    256: 269 / 59
+//   16 requests of 2000 tokens, 8 heads, head dim 128      16: 52 / 61   24: 69 / 63   32: 85 / 64   64: 153 / 65   256: 531 / 95   1024: 1932 / 238
+//   64 requests of 1000 tokens, 8 heads, head dim 128      16: 89 / 136  24: 127 / 138  32: 154 / 140  64: 284 / 141  256: 1023 / 183
+//   1 request of 16 000 tokens, 8 heads, head dim 128      16: 43 / 40   24: 48 / 43   32: 54 / 45   64: 83 / 46    256: 270 / 65
+//   16 requests of 2000 tokens, 8 heads, head dim 64       16: 43 / 51   24: 54 / 52   32: 68 / 54   64: 120 / 54
+//   16 requests of 2000 tokens, 8 heads, head dim 32       16: 39 / 49   24: 49 / 50   32: 62 / 52   64: 108 / 52   256: 376 / 68   1024: 1407 / 178
+//   64 requests of 1000 tokens, 8 heads, head dim 32       16: 64 / 103  24: 88 / 105  32: 113 / 107  64: 202 / 108  256: 720 / 128
 // It starts more slowly, which decides where there is little work (the lengths are not known here, the room in the tables is):
-//   1 request of 2000 tokens, 8 heads, head dim 128        32: 27 / 31  64: 28 / 32   128: 33 / 35  256: 50 / 44
-//   1 request of 300 tokens, 4 heads, head dim 64          64: 13 / 19  128: 13 / 20  256: 15 / 24
-// float16 turns at the same places (the second figures here and above are from before its row steps were pipelined: 0 to 15 % less now, at few columns the same):
-//   16 requests of 2000 tokens, 8 heads, head dim 128      16: 51 / 72   32: 84 / 75   64: 150 / 76   256: 529 / 100   1024: 2027 / 282
-//   1 request of 2000 tokens, 8 heads, head dim 128        32: 27 / 28  64: 28 / 30   128: 33 / 32  256: 50 / 38
-// and so do rows of 32 bytes (bfloat16):
-//   16 requests of 2000 tokens, 8 heads, head dim 32       16: 39 / 47   32: 61 / 51   64: 106 / 51   256: 375 / 64    1024: 1427 / 174
-//   64 requests of 1000 tokens, 8 heads, head dim 32       16: 64 / 88   32: 112 / 92  64: 201 / 92   256: 718 / 113
+//   1 request of 2000 tokens, 8 heads, head dim 128        32: 28 / 29  64: 28 / 30   128: 34 / 32  256: 50 / 39
+//   1 request of 300 tokens, 4 heads, head dim 64          64: 14 / 19  128: 14 / 20  256: 16 / 23
+// float16 turns at the same places:
+//   16 requests of 2000 tokens, 8 heads, head dim 128      16: 51 / 61   24: 69 / 62   32: 84 / 63   64: 151 / 64   256: 524 / 93    1024: 1909 / 236
+//   1 request of 2000 tokens, 8 heads, head dim 128        32: 27 / 28  64: 28 / 29   128: 34 / 32  256: 50 / 38
+// One kernel takes the whole batch, by its mean: single tokens beside a few prompt pieces go where the mean does.
 static bool many_queries(const SbCacheParams& p) {
     const int64_t columns = (int64_t)p.tokens * (p.heads / p.kv_heads);
     return p.dtype != SBATTN_F32 && p.ends && p.requests > 0 && columns >= 24 * (int64_t)p.requests &&

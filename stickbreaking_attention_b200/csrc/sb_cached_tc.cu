@@ -3,7 +3,7 @@
 //
 // A tile is two halves of 128 queries (rows of tensor memory) against the same keys, which take turns as in sb_tc_fwd_pair.cu: while the row threads of
 // one turn scores into weights, the tensor cores work for the other.  Codes become 16-bit operands once per block and step: keys float16 (exact; the queries
-// are scaled by a power of two per row to at most 2^15, exact too), values bfloat16 (exact).  The scale of the keys' page goes into the factor of a
+// are scaled by a power of two per row to at most 2^15, exact but for elements below 2^-31 of the row's largest, which lose 2^-39 of that), values bfloat16 (exact).  The scale of the keys' page goes into the factor of a
 // score, that of the values' page into the weight before that becomes two bfloat16 terms (2^-16 of it is lost; float16 weights would lack the range for scales
 // that differ from page to page), which the tensor cores multiply one after the other.  One term would do for bfloat16 results if all came from this kernel, as in
 // the forward kernels, and takes 198 us for 219 (below); but the same request comes here or to sb_cached.cu by what its batch looks like, and 2^-8 of the weights show
@@ -18,13 +18,14 @@
 // The product with the values starts with the right 64 keys while rows work on the left ones (173 -> 163 us at head dim 64, 160 -> 152 at 32, nothing at 128).
 // Tensor memory (512 columns): scores of the halves at 0 / 128 (the weights' two terms overwrite the scores of the same keys), sums at 256 / 384.
 //
-// Measured: 4 requests of 2000 ... 5000 tokens, 512 new ones each, 32 heads over 8, head dim 128: 195 us, 577 TFLOP/s (70 us at the rate of a bfloat16 GEMM), where
-// the kernel of sb_cached.cu takes 1 868. The special-function unit needs 2 560 cycles for a step of both halves, which takes about 5 500: issue slots are half busy,
-// the tensor pipe 30 %, and with a quarter of the conversions (head dim 32) a step is not much shorter. Rows wait for their own results. Codes straight from global memory to the operands, unrolled: 302 us; three warps that
-// convert keys and values, 168 registers: 386; codes by TMA and all loops rolled: 251; the rest is the queries' loads side by side, joins and shares.
-// float16, 4 requests of 4000 tokens, 512 new ones, the same heads: 226 us (bfloat16 205), in the kernel of sb_cached.cu 2 002.  Errors of 18
-// calls against float64 (2-norm, the output's own rounding is 2.1e-4): o as the plain form's; rem 2.18e-4 for its 2.13e-4 at 20 000 tokens, 2.33e-4 for 2.05e-4 at 60 000.
-// Head dim 32, the same requests and heads, bfloat16: 152 us, in the kernel of sb_cached.cu 1 408.
+// Measured: 4 requests of 2000 ... 5000 tokens, 512 new ones each, 32 heads over 8, head dim 128: 219 us, 514 TFLOP/s (70 us at the rate of a bfloat16 GEMM; the low terms, not
+// counted, are half as much again), where the kernel of sb_cached.cu takes 1 868. The special-function unit needs 2 560 cycles for a step of both halves, which takes about 6 100: issue slots
+// are busy 54 % of the time, the tensor pipe 42 %, and with a quarter of the conversions (head dim 32) a step is not much shorter. Rows wait for their own results. Earlier forms, with one
+// term of the weights: codes straight from global memory to the operands, unrolled: 302 us; three warps that convert keys and values, 168 registers: 386; codes by TMA and all
+// loops rolled: 251; the rest is the queries' loads side by side, joins and shares.
+// 4 requests of 4000 tokens, 512 new ones, the same heads: bfloat16 229 us, float16 227 (2 002 in the kernel of sb_cached.cu), head dim 64 188, 32 178 (1 408).  Errors of 18 calls of either
+// type against float64 (2-norm): bfloat16 as the plain form's, o and rem; float16 (the output's own rounding is 2.1e-4) o as the plain form's, rem 2.18e-4 for its 2.13e-4 at
+// 20 000 tokens, 2.33e-4 for 2.05e-4 at 60 000.
 #include <type_traits>
 
 #include "sb_cached.cuh"
