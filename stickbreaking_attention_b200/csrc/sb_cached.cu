@@ -18,7 +18,7 @@
 //     (22 bits: what is lost is below float32's own rounding of the sums), the two products are added to float32 accumulators.
 // float32 queries are two float16 terms, too; 16-bit ones are scaled by a power of two per row and exact (bfloat16: elements above 2^-31 of the row's largest).
 //
-// Measured (a copy's bandwidth is 6 551 GB/s): 32 requests of 1000 ... 12 000 tokens, 32 heads, head dim 128, 1.32 GB of codes 228-240 us, 5 500-5 800 GB/s; one request
+// Measured (a copy's bandwidth is 6 551 GB/s): 32 requests of 1000 ... 12 000 tokens, 32 heads, head dim 128, 1.32 GB of codes 222-240 us, 5 500-5 950 GB/s; one request
 // of 65 536 tokens, 8 heads 40 us, of which the steps take 18 (a bandwidth of 7 300 GB/s; what the loads cannot use is the start, lengths, tables, queries, and the
 // joins); 64 requests of 100 ... 4000 tokens, 8 heads of four queries each 46 us, 2 900 GB/s: four times the weights per key, and the steps' latency with three
 // warps a scheduler. Twelve warps with two stages each against eight with three: 239 / 284 us on the first (fewer spills, less to hide a step's latency with).
